@@ -1,0 +1,319 @@
+// kv8_abi.cpp -- the C ABI of the 8-bit paged cache (include/tq4_kv8.h): host
+// checks, split counts and launches.
+#include <hip/hip_runtime.h>
+
+#include "../../include/tq4.h"
+#include "../../include/tq4_kv8.h"
+#include "kv8_internal.hpp"
+
+namespace {
+
+constexpr uint32_t kStrip = 16;
+constexpr uint32_t kMaxPage = 1024;  // the writer's LDS map of a page's rows
+
+// A launch holds fewer than 2^32 work-items: so many workgroups of 256, and waves.
+constexpr uint64_t kMaxGroups = 0xffffffu;
+constexpr uint64_t kMaxWaves = 4 * kMaxGroups;
+
+int launched(hipError_t e) { return e == hipSuccess ? TQ4_OK : TQ4_ERR_LAUNCH; }
+
+bool aligned(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+// a * b * c held at 2^64 - 1
+uint64_t mul(uint64_t a, uint64_t b, uint64_t c = 1)
+{
+    uint64_t r;
+    if (__builtin_mul_overflow(a, b, &r) || __builtin_mul_overflow(r, c, &r)) return ~0ull;
+    return r;
+}
+
+int cache_checks(int element_type, int code_type, uint32_t num_kv_heads, uint32_t head_size,
+                 uint32_t block_size, uint32_t num_blocks)
+{
+    if (head_size != 64 && head_size != 128 && head_size != 256) return TQ4_ERR_HEAD_SIZE;
+    if ((element_type != 0 && element_type != 1) ||
+        (code_type != TQ4_KV8_FP8 && code_type != TQ4_KV8_INT8) || num_kv_heads == 0 ||
+        num_blocks == 0 || block_size == 0 || block_size % kStrip || block_size > kMaxPage)
+        return TQ4_ERR_GEOMETRY;
+    // slots are 32-bit; pages and heads are indexed in 32 bits too
+    if (mul(num_blocks, block_size) > 0x80000000ull || mul(num_blocks, num_kv_heads, 2) > 0xffffffffull)
+        return TQ4_ERR_RANGE;
+    return TQ4_OK;
+}
+
+struct Splits {
+    uint32_t K, kmin, wmin, wmax;
+};
+
+// How a sequence's tokens are cut (see kv8::split_width). items: (sequence, kv
+// head, row tile) triples of the call.
+Splits split_rule(uint64_t items, uint64_t cap, uint32_t num_splits)
+{
+    Splits s;
+    if (num_splits) {
+        s.kmin = s.K = num_splits;
+        s.wmin = 64;
+        s.wmax = 0x7fffffc0u;
+        return s;
+    }
+    // two workgroups a CU from full contexts, splits of at least 256 tokens (a
+    // wave's step each) and at most 1024 (a sixty-fourth of longer tables)
+    if (items == 0) items = 1;
+    uint64_t k = 512 / items;
+    s.kmin = (uint32_t)(k < 1 ? 1 : k > 64 ? 64 : k);
+    s.wmin = 256;
+    const uint64_t w = ((cap + 63) / 64 + 255) & ~255ull;
+    s.wmax = (uint32_t)(w < 1024 ? 1024 : w);
+    const uint64_t by_cap = (cap + s.wmax - 1) / s.wmax;
+    const uint64_t most = (cap + s.wmin - 1) / s.wmin;
+    if (s.kmin > most) s.kmin = (uint32_t)(most ? most : 1);
+    s.K = s.kmin > by_cap ? s.kmin : (uint32_t)by_cap;
+    if (s.K < 1) s.K = 1;
+    return s;
+}
+
+uint64_t tiles_of(uint64_t max_q, uint64_t group) { return (max_q * group + 15) / 16; }
+
+size_t record_bytes(uint64_t rows, uint64_t heads, uint32_t d, uint32_t K)
+{
+    if (K <= 1) return 0;
+    const uint64_t n = mul(rows, heads, K);
+    const uint64_t b = mul(n, (uint64_t)d + 2, sizeof(float));
+    return b > (uint64_t)SIZE_MAX - 16 ? SIZE_MAX : (size_t)((b + 15) & ~15ull);
+}
+
+int attention_checks(const void* q, const void* kc, const void* vc, const float* sc,
+                     const int32_t* tables, const int32_t* lens, const void* out,
+                     uint64_t q_stride, uint32_t rows, uint32_t num_seqs, uint32_t num_heads,
+                     uint32_t num_kv_heads, uint32_t head_size, uint32_t block_size,
+                     uint32_t max_blocks)
+{
+    if (num_heads == 0 || num_heads % num_kv_heads || num_heads / num_kv_heads > 16 ||
+        max_blocks == 0)
+        return TQ4_ERR_GEOMETRY;
+    if (mul(max_blocks, block_size) > 0x7fffffffull || rows > 0x7fffffffu ||
+        num_seqs > 0x7fffffffu || num_kv_heads > 65535u)
+        return TQ4_ERR_RANGE;
+    if (!q || !kc || !vc || !sc || !tables || !lens || !out) return TQ4_ERR_NULL_POINTER;
+    if (!aligned(q) || !aligned(kc) || !aligned(vc) || !aligned(out) || q_stride % 8)
+        return TQ4_ERR_ALIGNMENT;
+    if (rows > 1 && q_stride < (uint64_t)num_heads * head_size) return TQ4_ERR_GEOMETRY;
+    return TQ4_OK;
+}
+
+tq4::Kv8AttnParams make(const void* q, const void* kc, const void* vc, const float* sc,
+                        const int32_t* tables, const int32_t* lens, const int32_t* cu, void* out,
+                        uint64_t q_stride, uint32_t rows, uint32_t num_seqs, uint32_t num_heads,
+                        uint32_t num_kv_heads, uint32_t head_size, uint32_t block_size,
+                        uint32_t num_blocks, uint32_t max_blocks, uint32_t max_q, int causal,
+                        float scale, const Splits& s, void* workspace)
+{
+    tq4::Kv8AttnParams p{};
+    p.q = q;
+    p.key_cache = (const uint8_t*)kc;
+    p.value_cache = (const uint8_t*)vc;
+    p.scales = sc;
+    p.tables = tables;
+    p.context_lens = lens;
+    p.cu = cu;
+    p.acc = (float*)workspace;
+    p.ml = s.K > 1 ? p.acc + (uint64_t)rows * num_heads * s.K * head_size : nullptr;
+    p.out = out;
+    p.q_stride = q_stride;
+    p.rows = rows;
+    p.B = num_seqs;
+    p.Hq = num_heads;
+    p.Hkv = num_kv_heads;
+    p.G = num_heads / num_kv_heads;
+    p.D = head_size;
+    p.S = block_size;
+    p.P = num_blocks;
+    p.M = max_blocks;
+    p.K = s.K;
+    p.kmin = s.kmin;
+    p.wmin = s.wmin;
+    p.wmax = s.wmax;
+    p.max_q = max_q;
+    p.causal = causal;
+    p.scale = scale;
+    return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t tq4_paged_plan_workspace_bytes(uint32_t num_requests)
+{
+    return tq4::plan_workspace_bytes(num_requests);
+}
+
+int tq4_paged_plan(void* stream, const int32_t* context_lens, const int32_t* query_lens,
+                   const int32_t* release, int32_t* block_tables, int32_t* free_pages,
+                   const int32_t* free_state, int32_t* slot_mapping, int32_t* positions,
+                   int32_t* cu_seqlens, int32_t* granted, int32_t* new_context_lens,
+                   int32_t* new_free_state, void* workspace, size_t workspace_bytes,
+                   uint32_t num_requests, uint32_t max_blocks_per_seq, uint32_t block_size,
+                   uint32_t num_blocks, uint32_t max_tokens)
+{
+    if (num_requests == 0 || max_blocks_per_seq == 0 || num_blocks == 0 || block_size == 0 ||
+        block_size % kStrip)
+        return TQ4_ERR_GEOMETRY;
+    if (mul(num_blocks, block_size) > 0x80000000ull ||
+        mul(num_requests, max_blocks_per_seq) > 0x7fffffffull || max_tokens > 0x7fffffffu)
+        return TQ4_ERR_RANGE;
+    if (!context_lens || !query_lens || !block_tables || !free_pages || !free_state ||
+        (!slot_mapping && max_tokens) || !cu_seqlens || !granted || !new_context_lens || !new_free_state)
+        return TQ4_ERR_NULL_POINTER;
+    if (!workspace || !aligned(workspace) ||
+        workspace_bytes < tq4_paged_plan_workspace_bytes(num_requests))
+        return TQ4_ERR_WORKSPACE;
+    tq4::PlanParams p{};
+    p.context_lens = context_lens;
+    p.query_lens = query_lens;
+    p.release = release;
+    p.tables = block_tables;
+    p.ring = free_pages;
+    p.state = free_state;
+    p.slots = slot_mapping;
+    p.positions = positions;
+    p.cu = cu_seqlens;
+    p.granted = granted;
+    p.new_lens = new_context_lens;
+    p.new_state = new_free_state;
+    p.ws = (int32_t*)workspace;
+    p.B = num_requests;
+    p.M = max_blocks_per_seq;
+    p.S = block_size;
+    p.P = num_blocks;
+    p.T = max_tokens;
+    return launched(tq4::launch_plan((hipStream_t)stream, p));
+}
+
+int tq4_kv8_reshape_and_cache(void* stream, int element_type, int code_type, const void* key,
+                              const void* value, void* key_cache, void* value_cache,
+                              float* scale_cache, const int32_t* slot_mapping,
+                              uint64_t key_stride, uint64_t value_stride, uint32_t num_tokens,
+                              uint32_t num_kv_heads, uint32_t head_size, uint32_t block_size,
+                              uint32_t num_blocks)
+{
+    const int rc = cache_checks(element_type, code_type, num_kv_heads, head_size, block_size,
+                                num_blocks);
+    if (rc != TQ4_OK) return rc;
+    if (num_tokens == 0) return TQ4_OK;
+    if (mul(num_tokens, num_kv_heads, 2) > kMaxWaves) return TQ4_ERR_RANGE;
+    if (!key || !value || !key_cache || !value_cache || !scale_cache || !slot_mapping)
+        return TQ4_ERR_NULL_POINTER;
+    if (!aligned(key) || !aligned(value) || !aligned(key_cache) || !aligned(value_cache) ||
+        key_stride % 8 || value_stride % 8)
+        return TQ4_ERR_ALIGNMENT;
+    const uint64_t row = (uint64_t)num_kv_heads * head_size;
+    if (num_tokens > 1 && (key_stride < row || value_stride < row)) return TQ4_ERR_GEOMETRY;
+    tq4::Kv8WriteParams p{};
+    p.key = key;
+    p.value = value;
+    p.key_cache = (uint8_t*)key_cache;
+    p.value_cache = (uint8_t*)value_cache;
+    p.scales = scale_cache;
+    p.slots = slot_mapping;
+    p.key_stride = key_stride;
+    p.value_stride = value_stride;
+    p.T = num_tokens;
+    p.H = num_kv_heads;
+    p.D = head_size;
+    p.S = block_size;
+    p.P = num_blocks;
+    return launched(tq4::launch_kv8_writer((hipStream_t)stream, element_type,
+                                           code_type == TQ4_KV8_INT8, p));
+}
+
+size_t tq4_kv8_decode_workspace_bytes(uint32_t num_seqs, uint32_t num_heads,
+                                      uint32_t num_kv_heads, uint32_t head_size,
+                                      uint32_t block_size, uint32_t max_blocks_per_seq,
+                                      uint32_t num_splits)
+{
+    const Splits s = split_rule((uint64_t)num_seqs * num_kv_heads,
+                                (uint64_t)max_blocks_per_seq * block_size, num_splits);
+    return record_bytes(num_seqs, num_heads, head_size, s.K);
+}
+
+int tq4_kv8_paged_decode(void* stream, int element_type, int code_type, const void* q,
+                         const void* key_cache, const void* value_cache,
+                         const float* scale_cache, const int32_t* block_tables,
+                         const int32_t* context_lens, void* workspace, size_t workspace_bytes,
+                         void* out, uint64_t q_stride, uint32_t num_seqs, uint32_t num_heads,
+                         uint32_t num_kv_heads, uint32_t head_size, uint32_t block_size,
+                         uint32_t num_blocks, uint32_t max_blocks_per_seq, uint32_t num_splits,
+                         float scale)
+{
+    int rc = cache_checks(element_type, code_type, num_kv_heads, head_size, block_size, num_blocks);
+    if (rc != TQ4_OK) return rc;
+    if (num_seqs == 0) return TQ4_OK;
+    rc = attention_checks(q, key_cache, value_cache, scale_cache, block_tables, context_lens, out,
+                          q_stride, num_seqs, num_seqs, num_heads, num_kv_heads, head_size,
+                          block_size, max_blocks_per_seq);
+    if (rc != TQ4_OK) return rc;
+    if (num_splits > TQ4_KV8_MAX_SPLITS) return TQ4_ERR_SPLITS;
+    const Splits s = split_rule((uint64_t)num_seqs * num_kv_heads,
+                                (uint64_t)max_blocks_per_seq * block_size, num_splits);
+    const size_t need = record_bytes(num_seqs, num_heads, head_size, s.K);
+    if (need && (!workspace || !aligned(workspace) || workspace_bytes < need))
+        return TQ4_ERR_WORKSPACE;
+    if (mul(num_seqs, s.K) > kMaxGroups || mul(num_seqs, num_heads) > kMaxWaves)
+        return TQ4_ERR_RANGE;
+    return launched(tq4::launch_kv8_decode(
+        (hipStream_t)stream, element_type, code_type == TQ4_KV8_INT8,
+        make(q, key_cache, value_cache, scale_cache, block_tables, context_lens, nullptr, out,
+             q_stride, num_seqs, num_seqs, num_heads, num_kv_heads, head_size, block_size,
+             num_blocks, max_blocks_per_seq, 1, 1, scale, s, workspace)));
+}
+
+size_t tq4_kv8_prefill_workspace_bytes(uint32_t num_rows, uint32_t num_seqs, uint32_t num_heads,
+                                       uint32_t num_kv_heads, uint32_t head_size,
+                                       uint32_t block_size, uint32_t max_blocks_per_seq,
+                                       uint32_t max_query_len)
+{
+    if (num_kv_heads == 0) return 0;
+    if (max_query_len > num_rows) max_query_len = num_rows;
+    const uint64_t tiles = tiles_of(max_query_len, num_heads / num_kv_heads);
+    const Splits s = split_rule((uint64_t)num_seqs * num_kv_heads * tiles,
+                                (uint64_t)max_blocks_per_seq * block_size, 0);
+    return record_bytes(num_rows, num_heads, head_size, s.K);
+}
+
+int tq4_kv8_paged_prefill(void* stream, int element_type, int code_type, const void* q,
+                          const void* key_cache, const void* value_cache,
+                          const float* scale_cache, const int32_t* block_tables,
+                          const int32_t* context_lens, const int32_t* cu_seqlens,
+                          void* workspace, size_t workspace_bytes, void* out, uint64_t q_stride,
+                          uint32_t num_rows, uint32_t num_seqs, uint32_t num_heads,
+                          uint32_t num_kv_heads, uint32_t head_size, uint32_t block_size,
+                          uint32_t num_blocks, uint32_t max_blocks_per_seq,
+                          uint32_t max_query_len, int causal, float scale)
+{
+    int rc = cache_checks(element_type, code_type, num_kv_heads, head_size, block_size, num_blocks);
+    if (rc != TQ4_OK) return rc;
+    if (num_seqs == 0 || num_rows == 0 || max_query_len == 0) return TQ4_OK;
+    rc = attention_checks(q, key_cache, value_cache, scale_cache, block_tables, context_lens, out,
+                          q_stride, num_rows, num_seqs, num_heads, num_kv_heads, head_size,
+                          block_size, max_blocks_per_seq);
+    if (rc != TQ4_OK) return rc;
+    if (!cu_seqlens) return TQ4_ERR_NULL_POINTER;
+    if (max_query_len > num_rows) max_query_len = num_rows;
+    const uint64_t tiles = tiles_of(max_query_len, num_heads / num_kv_heads);
+    const Splits s = split_rule((uint64_t)num_seqs * num_kv_heads * tiles,
+                                (uint64_t)max_blocks_per_seq * block_size, 0);
+    const size_t need = record_bytes(num_rows, num_heads, head_size, s.K);
+    if (need && (!workspace || !aligned(workspace) || workspace_bytes < need))
+        return TQ4_ERR_WORKSPACE;
+    if (mul(num_seqs, s.K) > kMaxGroups || mul(num_rows, num_heads) > kMaxWaves ||
+        mul(num_kv_heads, tiles) > 65535u)
+        return TQ4_ERR_RANGE;
+    return launched(tq4::launch_kv8_decode(
+        (hipStream_t)stream, element_type, code_type == TQ4_KV8_INT8,
+        make(q, key_cache, value_cache, scale_cache, block_tables, context_lens, cu_seqlens, out,
+             q_stride, num_rows, num_seqs, num_heads, num_kv_heads, head_size, block_size,
+             num_blocks, max_blocks_per_seq, max_query_len, causal != 0, scale, s, workspace)));
+}
+
+}  // extern "C"

@@ -1,0 +1,114 @@
+// kv8_device.hpp -- device helpers of the attention over the 8-bit paged cache.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "kv8_internal.hpp"
+#include "tq4_device.hpp"
+
+namespace tq4 {
+namespace kv8 {
+
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNone = -3.0e38f;  // the running maximum before any token
+
+// Four codes of a word as f16 (exact for both types).
+template <int INT8>
+__device__ __forceinline__ void widen4(uint32_t w, h2_t& lo, h2_t& hi)
+{
+    if constexpr (INT8) {
+        // code + 128 in the low mantissa bits of 1024: 1024 + 128 + code
+        const uint32_t u = w ^ 0x80808080u;
+        const h2_t off = {(_Float16)1152.0f, (_Float16)1152.0f};
+        lo = __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off;
+        hi = __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off;
+    } else {
+        lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
+        hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
+    }
+}
+
+template <int INT8>
+__device__ __forceinline__ h8_t widen8(uint32_t w0, uint32_t w1)
+{
+    h2_t a, b, c, d;
+    widen4<INT8>(w0, a, b);
+    widen4<INT8>(w1, c, d);
+    return h8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+template <int BF16>
+__device__ __forceinline__ float widen_el(uint32_t bits16)
+{
+    if constexpr (BF16) return __uint_as_float(bits16 << 16);
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)bits16);
+}
+
+template <int BF16>
+__device__ __forceinline__ uint32_t narrow2(float a, float b)
+{
+    if constexpr (BF16) return f32_to_bf16(a) | f32_to_bf16(b) << 16;
+    const h2_t h = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, h);
+}
+
+__device__ __forceinline__ float held_scale(float s)
+{
+    return fminf(fmaxf(s, kKv8LeastScale), kKv8MostScale);
+}
+
+// x scaled so that a row whose largest magnitude is `most` lies in f16's normal
+// range: the power of two that brings it to [1, 2) (1 for a row of zeros).
+__device__ __forceinline__ float row_shift(float most)
+{
+    const uint32_t e = (__float_as_uint(most) >> 23) & 0xffu;
+    return e == 0u ? (most > 0.0f ? 0x1.0p+126f : 1.0f)
+                   : __uint_as_float((254u - (e > 253u ? 253u : e)) << 23);
+}
+
+// n / d for n < 2^31 by the multiplier of div_magic.
+struct Divisor {
+    uint32_t magic, shift;
+};
+__device__ __forceinline__ uint32_t div_by(uint32_t n, Divisor d)
+{
+    return (uint32_t)(((uint64_t)n * d.magic) >> d.shift);
+}
+inline Divisor div_magic(uint32_t d)
+{
+    uint32_t shift = 31;
+    while (shift < 63 && (1ull << (shift - 31)) < d) ++shift;
+    return {d == 1 ? 0x80000000u : (uint32_t)((1ull << shift) / d + 1), shift};
+}
+
+// The tokens that a split of a sequence of L tokens holds (a multiple of 64):
+// L cut into kmin parts, none longer than wmax.
+__device__ __forceinline__ uint32_t split_width(uint32_t L, uint32_t kmin, uint32_t wmin,
+                                                uint32_t wmax)
+{
+    uint32_t w = ((L + kmin - 1) / kmin + 63u) & ~63u;
+    if (w < wmin) w = wmin;
+    return w < wmax ? w : wmax;
+}
+
+// All 16 bytes of a strip's channel with those of dead tokens (>= live) zero.
+__device__ __forceinline__ u4_t live_bytes(u4_t v, int live)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int n = live - 4 * i;
+        const uint32_t m = n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+        v[i] &= m;
+    }
+    return v;
+}
+
+}  // namespace kv8
+}  // namespace tq4

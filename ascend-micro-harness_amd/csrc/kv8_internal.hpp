@@ -1,0 +1,53 @@
+// kv8_internal.hpp -- launches of the 8-bit paged cache's kernels (tq4_kv8.h),
+// called by kv8_abi.cpp after its checks.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace tq4 {
+
+constexpr float kKv8LeastScale = 0x1.0p-100f;
+constexpr float kKv8MostScale = 0x1.0p+120f;
+
+struct PlanParams {
+    const int32_t *context_lens, *query_lens, *release;
+    int32_t *tables, *ring;
+    const int32_t* state;
+    int32_t *slots, *positions, *cu, *granted, *new_lens, *new_state;
+    int32_t* ws;
+    uint32_t B, M, S, P, T;
+};
+size_t plan_workspace_bytes(uint32_t B);
+hipError_t launch_plan(hipStream_t stream, const PlanParams& p);
+
+struct Kv8WriteParams {
+    const void *key, *value;
+    uint8_t *key_cache, *value_cache;
+    float* scales;
+    const int32_t* slots;
+    uint64_t key_stride, value_stride;
+    uint32_t T, H, D, S, P;
+};
+hipError_t launch_kv8_writer(hipStream_t stream, int bf16, int int8, const Kv8WriteParams& p);
+
+// Attention. Split k of a sequence of L tokens holds tokens [k*W, (k+1)*W), W
+// = split_width(L, ..) (kv8_device.hpp); cu NULL: one row a sequence.
+struct Kv8AttnParams {
+    const void* q;
+    const uint8_t *key_cache, *value_cache;
+    const float* scales;
+    const int32_t *tables, *context_lens, *cu;
+    float *acc, *ml;  // records: [row][K][D] and [row][K][2], row = q row * Hq + head
+    void* out;
+    uint64_t q_stride;
+    uint32_t rows, B, Hq, Hkv, G, D, S, P, M;
+    uint32_t K, kmin, wmin, wmax;  // splits, see split_width
+    uint32_t max_q;
+    int causal;
+    float scale;
+};
+hipError_t launch_kv8_decode(hipStream_t stream, int bf16, int int8, const Kv8AttnParams& p);
+hipError_t launch_kv8_prefill(hipStream_t stream, int bf16, int int8, const Kv8AttnParams& p);
+
+}  // namespace tq4

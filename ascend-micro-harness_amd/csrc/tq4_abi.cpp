@@ -84,6 +84,7 @@ const char* tq4_status_string(int status)
         case TQ4_ERR_FLAGS: return "unknown flag bits, or a test hook without its poll bound";
         case TQ4_ERR_SCRATCH:
             return "the call needs more than the no-allocation entry's 16 MiB static scratch";
+        case TQ4_ERR_ALIGNMENT: return "a buffer or a row stride is not 16-byte aligned";
         default: return "unknown status";
     }
 }

@@ -23,6 +23,7 @@
 
 #include "../../include/tq4.h"
 #include "../../include/tq4_kv4fp8.h"
+#include "../../include/tq4_kv8.h"
 
 namespace {
 
@@ -40,6 +41,13 @@ struct Abi {
     decltype(&tq4_kv4fp8_workspace_bytes) kv4fp8_workspace_bytes;
     decltype(&tq4_kv4fp8_decode) kv4fp8_decode;
     decltype(&tq4_kv4fp8_decode_raw_query) kv4fp8_decode_raw_query;
+    decltype(&tq4_paged_plan_workspace_bytes) paged_plan_workspace_bytes;
+    decltype(&tq4_paged_plan) paged_plan;
+    decltype(&tq4_kv8_reshape_and_cache) kv8_reshape_and_cache;
+    decltype(&tq4_kv8_decode_workspace_bytes) kv8_decode_workspace_bytes;
+    decltype(&tq4_kv8_paged_decode) kv8_paged_decode;
+    decltype(&tq4_kv8_prefill_workspace_bytes) kv8_prefill_workspace_bytes;
+    decltype(&tq4_kv8_paged_prefill) kv8_paged_prefill;
 };
 Abi g_abi;
 bool g_bound = false;
@@ -599,6 +607,273 @@ PyObject* lloydmax_quantize(PyObject*, PyObject* const* a, Py_ssize_t n)
     });
 }
 
+// ------------------------------------------------------- the 8-bit paged cache
+constexpr uint32_t kCodes8 = bit(at::kFloat8_e4m3fn) | bit(at::kChar);
+
+// The calls of kv8.py take tensors of one GPU; the native path takes those of
+// the current one, on its current stream (stream None).
+struct Kv8Args : Args {
+    int device = -1;
+
+    const at::Tensor* on(const at::Tensor* t)
+    {
+        if (!t) return nullptr;
+        if (device < 0) device = t->get_device();
+        else if (t->get_device() != device) ok = false;
+        return t;
+    }
+    const at::Tensor* in(uint32_t dtypes) { return on(tensor(dtypes)); }
+    const at::Tensor* in_or_none(uint32_t dtypes) { return on(tensor_or_none(dtypes)); }
+    // activations [rows][heads][d], rows contiguous and apart
+    const at::Tensor* rows(uint32_t dtypes, Shape3& s, uint64_t& stride)
+    {
+        PyObject* o = next();
+        if (!ok || !THPVariable_CheckExact(o)) return ok = false, nullptr;
+        const at::Tensor& t = THPVariable_Unpack(o);
+        if (!t.defined() || t.layout() != at::kStrided || !t.has_storage() || !t.is_cuda() ||
+            (int)t.scalar_type() >= 32 || !((dtypes >> (int)t.scalar_type()) & 1u) ||
+            !shape3(&t, s))
+            return ok = false, nullptr;
+        const int64_t row = s.b * s.c;
+        if ((s.b > 1 && t.stride(1) != s.c) || (s.c > 1 && t.stride(2) != 1) ||
+            (s.a > 1 && t.stride(0) < row))
+            return ok = false, nullptr;
+        stride = (uint64_t)(s.a > 1 ? t.stride(0) : row);
+        return on(&t);
+    }
+    void* current_stream()
+    {
+        if (!need(next() == Py_None && device >= 0 &&
+                  device == (int)c10::hip::current_device()))
+            return nullptr;
+        return (void*)c10::hip::getCurrentHIPStream().stream();
+    }
+};
+
+template <class F>
+PyObject* entry8(PyObject* const* a, Py_ssize_t n, F&& f)
+{
+    return entry(a, n, [&](Args& g) -> PyObject* {
+        Kv8Args k{g};
+        return f(k);
+    });
+}
+
+at::Tensor bytes_like(const at::Tensor* t, size_t n)
+{
+    return at::empty({(int64_t)n}, t->options().dtype(at::kByte));
+}
+
+// A cache's sizes and its three tensors (kv8.py _pool).
+struct Pool8 {
+    const at::Tensor *kc, *vc, *sc;
+    uint32_t P = 0, H = 0, S = 0, d = 0;
+    int code = 0;
+
+    explicit Pool8(Kv8Args& g) : kc(g.in(kCodes8)), vc(g.in(kCodes8)), sc(g.in(kF32))
+    {
+        if (!g.need(kc && vc && sc && kc->dim() == 4 && kc->numel() > 0 &&
+                    vc->scalar_type() == kc->scalar_type() && vc->numel() == kc->numel() &&
+                    small(kc->size(0)) && small(kc->size(1)) && small(kc->size(2)) &&
+                    small(kc->size(3)) &&
+                    (uint64_t)sc->numel() == mul(mul(kc->size(0), kc->size(1)), 2)))
+            return;
+        P = (uint32_t)kc->size(0);
+        H = (uint32_t)kc->size(1);
+        S = (uint32_t)kc->size(2);
+        d = (uint32_t)kc->size(3);
+        code = kc->scalar_type() == at::kChar ? TQ4_KV8_INT8 : TQ4_KV8_FP8;
+    }
+};
+
+bool holds_all(const at::Tensor* t, int64_t n) { return t && t->numel() == n; }
+
+// (context_lens, query_lens, block_tables, free_pages, free_state, slot_mapping,
+//  cu_seqlens, granted, block_size, release, positions, new_context_lens,
+//  new_free_state, workspace, stream)
+PyObject* paged_plan(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return entry8(a, n, [](Kv8Args& g) -> PyObject* {
+        const at::Tensor *cl = g.in(kI32), *ql = g.in(kI32), *bt = g.in(kI32), *ring = g.in(kI32),
+                         *state = g.in(kI32), *slots = g.in(kI32), *cu = g.in(kI32),
+                         *granted = g.in(kI32);
+        const uint32_t S = g.num();
+        const at::Tensor *release = g.in_or_none(kI32), *pos = g.in_or_none(kI32),
+                         *ncl = g.in_or_none(kI32), *nstate = g.in_or_none(kI32),
+                         *ws = g.in_or_none(~0u);
+        void* st = g.current_stream();
+        if (!g.need(bt && bt->dim() == 2 && bt->numel() > 0 && small(bt->size(0)) &&
+                    small(bt->size(1))))
+            return nullptr;
+        const int64_t B = bt->size(0);
+        if (!g.need(holds_all(cl, B) && holds_all(ql, B) && holds_all(state, 2) &&
+                    holds_all(cu, B + 1) && holds_all(granted, B) && ring && ring->numel() > 0 &&
+                    small(ring->numel()) && slots && small(slots->numel()) &&
+                    (!release || holds_all(release, B)) &&
+                    (!pos || holds_all(pos, slots->numel())) && (!ncl || holds_all(ncl, B)) &&
+                    (!nstate || holds_all(nstate, 2))))
+            return nullptr;
+        at::Tensor fresh;
+        if (!ws) {
+            fresh = bytes_like(bt, g_abi.paged_plan_workspace_bytes((uint32_t)B));
+            ws = &fresh;
+        }
+        return PyLong_FromLong(unlocked([&] {
+            return g_abi.paged_plan(
+                st, (const int32_t*)ptr(cl), (const int32_t*)ptr(ql), (const int32_t*)ptr(release),
+                (int32_t*)ptr(bt), (int32_t*)ptr(ring), (const int32_t*)ptr(state),
+                (int32_t*)ptr(slots), (int32_t*)ptr(pos), (int32_t*)ptr(cu),
+                (int32_t*)ptr(granted), (int32_t*)ptr(ncl ? ncl : cl),
+                (int32_t*)ptr(nstate ? nstate : state), ptr(ws), nbytes(ws), (uint32_t)B,
+                (uint32_t)bt->size(1), S, (uint32_t)ring->numel(), (uint32_t)slots->numel());
+        }));
+    });
+}
+
+// (key, value, key_cache, value_cache, scale_cache, slot_mapping, stream)
+PyObject* kv8_reshape_and_cache(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return entry8(a, n, [](Kv8Args& g) -> PyObject* {
+        Shape3 s{}, sv{};
+        uint64_t ks = 0, vs = 0;
+        const at::Tensor* k = g.rows(kBf16 | kF16, s, ks);
+        if (!k) return nullptr;
+        const at::Tensor* v = g.rows(bit(k->scalar_type()), sv, vs);
+        const Pool8 c(g);
+        const at::Tensor* sl = g.in(kI32);
+        void* st = g.current_stream();
+        if (!g.need(v && sv.a == s.a && sv.b == s.b && sv.c == s.c && s.b == c.H && s.c == c.d &&
+                    at_least(sl, (uint64_t)s.a)))
+            return nullptr;
+        return PyLong_FromLong(unlocked([&] {
+            return g_abi.kv8_reshape_and_cache(
+                st, k->scalar_type() == at::kBFloat16, c.code, ptr(k), ptr(v), ptr(c.kc),
+                ptr(c.vc), (float*)ptr(c.sc), (const int32_t*)ptr(sl), ks, vs, (uint32_t)s.a, c.H,
+                c.d, c.S, c.P);
+        }));
+    });
+}
+
+// What the two attention entries share, up to their own arguments.
+struct Attention8 {
+    Shape3 s{};
+    uint64_t stride = 0;
+    const at::Tensor* q;
+    Pool8 c;
+    const at::Tensor *bt, *cl;
+    uint32_t B = 0, M = 0;
+
+    explicit Attention8(Kv8Args& g)
+        : q(g.rows(kBf16 | kF16, s, stride)), c(g), bt(g.in(kI32)), cl(g.in(kI32))
+    {
+        if (!g.need(q && bt && bt->dim() == 2 && bt->numel() > 0 && small(bt->size(0)) &&
+                    small(bt->size(1)) && s.c == c.d && holds_all(cl, bt->size(0))))
+            return;
+        B = (uint32_t)bt->size(0);
+        M = (uint32_t)bt->size(1);
+    }
+    int element() const { return q->scalar_type() == at::kBFloat16; }
+};
+
+// The output argument: a tensor of q's type and size, or None (out is null and
+// `made` is filled before the launch).
+struct Out8 {
+    PyObject* given;
+    const at::Tensor* t;
+
+    Out8(Kv8Args& g, const Attention8& x) : given(g.next()), t(nullptr)
+    {
+        if (!g.ok || given == Py_None) return;
+        t = g.on(plain(given, bit(x.q->scalar_type())));
+        g.need(t && t->numel() == x.q->numel());
+    }
+    void make(const Attention8& x, at::Tensor& made)
+    {
+        if (t) return;
+        made = at::empty({x.s.a, x.s.b, x.s.c}, x.q->options());
+        t = &made;
+    }
+    PyObject* result(int rc, const at::Tensor& made)
+    {
+        if (rc != 0) return PyLong_FromLong(rc);
+        if (made.defined()) return THPVariable_Wrap(made);
+        Py_INCREF(given);
+        return given;
+    }
+};
+
+// (q, key_cache, value_cache, scale_cache, block_tables, context_lens, out,
+//  workspace, num_splits, scale, stream)
+PyObject* kv8_paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return entry8(a, n, [](Kv8Args& g) -> PyObject* {
+        const Attention8 x(g);
+        if (!g.ok) return nullptr;
+        Out8 out(g, x);
+        const at::Tensor* ws = g.in_or_none(~0u);
+        const uint32_t K = g.num();
+        const float scale = g.real(inv_sqrt(x.s.c));
+        void* st = g.current_stream();
+        if (!g.need(x.s.a == x.B && K <= TQ4_KV8_MAX_SPLITS && small(x.s.b))) return nullptr;
+        const uint32_t Hq = (uint32_t)x.s.b;
+        at::Tensor made, room;
+        out.make(x, made);
+        if (!ws) {
+            const size_t need = g_abi.kv8_decode_workspace_bytes(x.B, Hq, x.c.H, x.c.d, x.c.S,
+                                                                 x.M, K);
+            if (need) {
+                room = bytes_like(x.q, need);
+                ws = &room;
+            }
+        }
+        const int rc = unlocked([&] {
+            return g_abi.kv8_paged_decode(
+                st, x.element(), x.c.code, ptr(x.q), ptr(x.c.kc), ptr(x.c.vc),
+                (const float*)ptr(x.c.sc), (const int32_t*)ptr(x.bt), (const int32_t*)ptr(x.cl),
+                ptr(ws), nbytes(ws), ptr(out.t), x.stride, x.B, Hq, x.c.H, x.c.d, x.c.S, x.c.P,
+                x.M, K, scale);
+        });
+        return out.result(rc, made);
+    });
+}
+
+// (q, key_cache, value_cache, scale_cache, block_tables, context_lens,
+//  cu_seqlens, max_query_len, causal, out, workspace, scale, stream)
+PyObject* kv8_paged_prefill(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return entry8(a, n, [](Kv8Args& g) -> PyObject* {
+        const Attention8 x(g);
+        const at::Tensor* cu = g.in(kI32);
+        const uint32_t longest = g.num();
+        const bool causal = g.flag();
+        if (!g.ok) return nullptr;
+        Out8 out(g, x);
+        const at::Tensor* ws = g.in_or_none(~0u);
+        const float scale = g.real(inv_sqrt(x.s.c));
+        void* st = g.current_stream();
+        if (!g.need(holds_all(cu, (int64_t)x.B + 1))) return nullptr;
+        const uint32_t Hq = (uint32_t)x.s.b, T = (uint32_t)x.s.a;
+        at::Tensor made, room;
+        out.make(x, made);
+        if (!ws) {
+            const size_t need = g_abi.kv8_prefill_workspace_bytes(T, x.B, Hq, x.c.H, x.c.d, x.c.S,
+                                                                  x.M, longest);
+            if (need) {
+                room = bytes_like(x.q, need);
+                ws = &room;
+            }
+        }
+        const int rc = unlocked([&] {
+            return g_abi.kv8_paged_prefill(
+                st, x.element(), x.c.code, ptr(x.q), ptr(x.c.kc), ptr(x.c.vc),
+                (const float*)ptr(x.c.sc), (const int32_t*)ptr(x.bt), (const int32_t*)ptr(x.cl),
+                (const int32_t*)ptr(cu), ptr(ws), nbytes(ws), ptr(out.t), x.stride, T, x.B, Hq,
+                x.c.H, x.c.d, x.c.S, x.c.P, x.M, longest, causal, scale);
+        });
+        return out.result(rc, made);
+    });
+}
+
 // bind({name: address}) -- the loaded library's entries
 PyObject* bind(PyObject*, PyObject* arg)
 {
@@ -620,6 +895,13 @@ PyObject* bind(PyObject*, PyObject* arg)
         {"tq4_kv4fp8_workspace_bytes", (void**)&g_abi.kv4fp8_workspace_bytes},
         {"tq4_kv4fp8_decode", (void**)&g_abi.kv4fp8_decode},
         {"tq4_kv4fp8_decode_raw_query", (void**)&g_abi.kv4fp8_decode_raw_query},
+        {"tq4_paged_plan_workspace_bytes", (void**)&g_abi.paged_plan_workspace_bytes},
+        {"tq4_paged_plan", (void**)&g_abi.paged_plan},
+        {"tq4_kv8_reshape_and_cache", (void**)&g_abi.kv8_reshape_and_cache},
+        {"tq4_kv8_decode_workspace_bytes", (void**)&g_abi.kv8_decode_workspace_bytes},
+        {"tq4_kv8_paged_decode", (void**)&g_abi.kv8_paged_decode},
+        {"tq4_kv8_prefill_workspace_bytes", (void**)&g_abi.kv8_prefill_workspace_bytes},
+        {"tq4_kv8_paged_prefill", (void**)&g_abi.kv8_paged_prefill},
     };
     for (const auto& e : all) {
         PyObject* v = PyDict_GetItemString(arg, e.name);
@@ -641,6 +923,10 @@ PyMethodDef kMethods[] = {TQ4_FAST(reshape_and_cache),
                           TQ4_FAST(kv4fp8_decode),
                           TQ4_FAST(icdf_quantize),
                           TQ4_FAST(lloydmax_quantize),
+                          TQ4_FAST(paged_plan),
+                          TQ4_FAST(kv8_reshape_and_cache),
+                          TQ4_FAST(kv8_paged_decode),
+                          TQ4_FAST(kv8_paged_prefill),
                           {"bind", bind, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_tq4_host",

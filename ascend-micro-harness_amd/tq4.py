@@ -146,7 +146,9 @@ def _bind_host(L):
             "tq4_decode_auto_splits", "tq4_paged_decode", "tq4_paged_decode_partials",
             "tq4_splitk_combine", "tq4_rms_reshape_and_cache", "tq4_icdf_quantize",
             "tq4_lloydmax_quantize", "tq4_kv4fp8_workspace_bytes", "tq4_kv4fp8_decode",
-            "tq4_kv4fp8_decode_raw_query")})
+            "tq4_kv4fp8_decode_raw_query", "tq4_paged_plan_workspace_bytes", "tq4_paged_plan",
+            "tq4_kv8_reshape_and_cache", "tq4_kv8_decode_workspace_bytes", "tq4_kv8_paged_decode",
+            "tq4_kv8_prefill_workspace_bytes", "tq4_kv8_paged_prefill")})
     except ImportError as e:
         warnings.warn(f"_tq4_host is not used: {e}; build it again (make -C csrc host) or remove it",
                       RuntimeWarning, stacklevel=3)

@@ -48,7 +48,8 @@ typedef enum {
     TQ4_ERR_RANGE = -10,        /* a size exceeds what the kernels index */
     TQ4_ERR_CODEBOOK = -11,     /* codebook leaf: bits, mode or element count */
     TQ4_ERR_FLAGS = -12,        /* unknown flag bits, or a test hook without its bound */
-    TQ4_ERR_SCRATCH = -13       /* beyond the no-allocation entry's static scratch */
+    TQ4_ERR_SCRATCH = -13,      /* beyond the no-allocation entry's static scratch */
+    TQ4_ERR_ALIGNMENT = -14     /* tq4_kv8.h: a buffer or a row stride off 16 bytes */
 } tq4_status;
 
 /* Human-readable name of a tq4_status. */
