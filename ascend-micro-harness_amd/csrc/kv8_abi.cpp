@@ -201,7 +201,7 @@ int tq4_kv8_reshape_and_cache(void* stream, int element_type, int code_type, con
                                 num_blocks);
     if (rc != TQ4_OK) return rc;
     if (num_tokens == 0) return TQ4_OK;
-    if (mul(num_tokens, num_kv_heads, 2) > kMaxWaves) return TQ4_ERR_RANGE;
+    if (num_kv_heads > 8192u || mul(num_tokens, num_kv_heads) > (1u << 26)) return TQ4_ERR_RANGE;
     if (!key || !value || !key_cache || !value_cache || !scale_cache || !slot_mapping)
         return TQ4_ERR_NULL_POINTER;
     if (!aligned(key) || !aligned(value) || !aligned(key_cache) || !aligned(value_cache) ||

@@ -97,7 +97,8 @@ int tq4_paged_plan(void* stream, const int32_t* context_lens, const int32_t* que
  * offsets; of two rows for one slot the later one is written, the other counts
  * for nothing. Rows of one page in
  * two places of a call leave that page's codes and scale undefined (no other
- * page's). num_tokens * num_kv_heads < 2^25 (TQ4_ERR_RANGE). */
+ * page's). num_kv_heads <= 8192, num_tokens * num_kv_heads <= 2^26
+ * (TQ4_ERR_RANGE). */
 int tq4_kv8_reshape_and_cache(void* stream, int element_type, int code_type, const void* key,
                               const void* value, void* key_cache, void* value_cache,
                               float* scale_cache, const int32_t* slot_mapping,

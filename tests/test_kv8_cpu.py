@@ -47,7 +47,7 @@ def test_writer_refusals(lib):
     assert call(d=96) == -2
     assert call(el=2) == call(code=2) == call(H=0) == call(P=0) == call(S=24) == call(S=1040) == -3
     assert call(ks=128) == call(vs=248) == -3
-    assert call(P=2 ** 28) == call(T=2 ** 25, ks=512, H=1) == -10
+    assert call(P=2 ** 28) == call(T=2 ** 27, H=1) == call(H=8193) == -10
     assert call(key=None) == -1
     assert call(key=ODD) == call(kc=ODD) == call(ks=260) == -14
     assert call(T=0) == 0
