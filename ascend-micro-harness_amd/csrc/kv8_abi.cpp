@@ -11,9 +11,8 @@ namespace {
 constexpr uint32_t kStrip = 16;
 constexpr uint32_t kMaxPage = 1024;  // the writer's LDS map of a page's rows
 
-// A launch holds fewer than 2^32 work-items: so many workgroups of 256, and waves.
+// A launch holds fewer than 2^32 work-items: so many workgroups of 256.
 constexpr uint64_t kMaxGroups = 0xffffffu;
-constexpr uint64_t kMaxWaves = 4 * kMaxGroups;
 
 int launched(hipError_t e) { return e == hipSuccess ? TQ4_OK : TQ4_ERR_LAUNCH; }
 
@@ -41,45 +40,59 @@ int cache_checks(int element_type, int code_type, uint32_t num_kv_heads, uint32_
     return TQ4_OK;
 }
 
-struct Splits {
-    uint32_t K, kmin, wmin, wmax;
+// How a call's work is cut (kv8_decode.hip): K parts a sequence, or 0: streamed
+// over `groups` workgroups.
+struct Cut {
+    uint32_t K, groups, least;
 };
 
-// How a sequence's tokens are cut (see kv8::split_width). items: (sequence, kv
-// head, row tile) triples of the call.
-Splits split_rule(uint64_t items, uint64_t cap, uint32_t num_splits)
+uint64_t tiles_of(uint64_t max_q, uint64_t group)
 {
-    Splits s;
-    if (num_splits) {
-        s.kmin = s.K = num_splits;
-        s.wmin = 64;
-        s.wmax = 0x7fffffc0u;
-        return s;
-    }
-    // two workgroups a CU from full contexts, splits of at least 256 tokens (a
-    // wave's step each) and at most 1024 (a sixty-fourth of longer tables)
-    if (items == 0) items = 1;
-    uint64_t k = 512 / items;
-    s.kmin = (uint32_t)(k < 1 ? 1 : k > 64 ? 64 : k);
-    s.wmin = 256;
-    const uint64_t w = ((cap + 63) / 64 + 255) & ~255ull;
-    s.wmax = (uint32_t)(w < 1024 ? 1024 : w);
-    const uint64_t by_cap = (cap + s.wmax - 1) / s.wmax;
-    const uint64_t most = (cap + s.wmin - 1) / s.wmin;
-    if (s.kmin > most) s.kmin = (uint32_t)(most ? most : 1);
-    s.K = s.kmin > by_cap ? s.kmin : (uint32_t)by_cap;
-    if (s.K < 1) s.K = 1;
-    return s;
+    return (max_q * group + tq4::kKv8Rows - 1) / tq4::kKv8Rows;
 }
 
-uint64_t tiles_of(uint64_t max_q, uint64_t group) { return (max_q * group + 15) / 16; }
-
-size_t record_bytes(uint64_t rows, uint64_t heads, uint32_t d, uint32_t K)
+// Tables of up to 1024 tokens are not worth a second kernel: one workgroup an
+// item. One sequence: even parts, of 256 tokens (a unit a wave) at least. Several:
+// streamed over as many workgroups as the CUs hold, at least four units each.
+Cut cut_rule(uint32_t d, uint64_t seqs, uint64_t heads, uint64_t tiles, uint64_t cap,
+             uint32_t num_splits)
 {
-    if (K <= 1) return 0;
-    const uint64_t n = mul(rows, heads, K);
-    const uint64_t b = mul(n, (uint64_t)d + 2, sizeof(float));
+    Cut c{num_splits, 0, 4};
+    if (num_splits) return c;
+    c.groups = 256u * (uint32_t)tq4::kKv8GroupsPerCu((int)d);
+    if (cap <= 1024) {
+        c.K = 1;
+    } else if (seqs == 1) {
+        const uint64_t items = heads * tiles ? heads * tiles : 1;
+        uint64_t k = c.groups / items;
+        if (k > (cap + 255) / 256) k = (cap + 255) / 256;
+        if (k > TQ4_KV8_MAX_SPLITS) k = TQ4_KV8_MAX_SPLITS;
+        c.K = (uint32_t)(k ? k : 1);
+    }
+    return c;
+}
+
+uint32_t record_rows(uint64_t max_q, uint64_t group)
+{
+    return (uint32_t)(max_q * group < tq4::kKv8Rows ? max_q * group : tq4::kKv8Rows);
+}
+
+// Records of a call: (floats of a row's sums, and two statistics) a row and slot.
+uint64_t record_slots(const Cut& c, uint64_t items)
+{
+    return c.K == 1 ? 0 : c.K ? mul(items, c.K) : 2ull * c.groups;
+}
+size_t record_bytes(const Cut& c, uint64_t items, uint32_t rec_rows, uint32_t d)
+{
+    const uint64_t b = mul(mul(record_slots(c, items), rec_rows), (uint64_t)d + 2, sizeof(float));
     return b > (uint64_t)SIZE_MAX - 16 ? SIZE_MAX : (size_t)((b + 15) & ~15ull);
+}
+
+// The grid and the line of a streamed call's units in bounds.
+bool cut_fits(const Cut& c, uint64_t seqs, uint64_t cap, uint64_t heads, uint64_t tiles)
+{
+    if (c.K) return mul(seqs, c.K) <= kMaxGroups && mul(heads, tiles) <= 65535u;
+    return mul(mul(seqs, (cap + tq4::kKv8Unit - 1) / tq4::kKv8Unit), heads, tiles) <= 0xff000000ull;
 }
 
 int attention_checks(const void* q, const void* kc, const void* vc, const float* sc,
@@ -106,7 +119,7 @@ tq4::Kv8AttnParams make(const void* q, const void* kc, const void* vc, const flo
                         uint64_t q_stride, uint32_t rows, uint32_t num_seqs, uint32_t num_heads,
                         uint32_t num_kv_heads, uint32_t head_size, uint32_t block_size,
                         uint32_t num_blocks, uint32_t max_blocks, uint32_t max_q, int causal,
-                        float scale, const Splits& s, void* workspace)
+                        float scale, const Cut& cut, void* workspace)
 {
     tq4::Kv8AttnParams p{};
     p.q = q;
@@ -116,8 +129,12 @@ tq4::Kv8AttnParams make(const void* q, const void* kc, const void* vc, const flo
     p.tables = tables;
     p.context_lens = lens;
     p.cu = cu;
+    p.rec_rows = record_rows(max_q, num_heads / num_kv_heads);
     p.acc = (float*)workspace;
-    p.ml = s.K > 1 ? p.acc + (uint64_t)rows * num_heads * s.K * head_size : nullptr;
+    const uint64_t items = (uint64_t)num_seqs * num_kv_heads *
+                           tiles_of(max_q, num_heads / num_kv_heads);
+    if (const uint64_t slots = record_slots(cut, items))
+        p.ml = p.acc + slots * p.rec_rows * head_size;
     p.out = out;
     p.q_stride = q_stride;
     p.rows = rows;
@@ -129,10 +146,9 @@ tq4::Kv8AttnParams make(const void* q, const void* kc, const void* vc, const flo
     p.S = block_size;
     p.P = num_blocks;
     p.M = max_blocks;
-    p.K = s.K;
-    p.kmin = s.kmin;
-    p.wmin = s.wmin;
-    p.wmax = s.wmax;
+    p.K = cut.K;
+    p.groups = cut.groups;
+    p.least = cut.least;
     p.max_q = max_q;
     p.causal = causal;
     p.scale = scale;
@@ -232,9 +248,11 @@ size_t tq4_kv8_decode_workspace_bytes(uint32_t num_seqs, uint32_t num_heads,
                                       uint32_t block_size, uint32_t max_blocks_per_seq,
                                       uint32_t num_splits)
 {
-    const Splits s = split_rule((uint64_t)num_seqs * num_kv_heads,
-                                (uint64_t)max_blocks_per_seq * block_size, num_splits);
-    return record_bytes(num_seqs, num_heads, head_size, s.K);
+    if (num_kv_heads == 0) return 0;
+    const Cut c = cut_rule(head_size, num_seqs, num_kv_heads, 1,
+                           (uint64_t)max_blocks_per_seq * block_size, num_splits);
+    return record_bytes(c, (uint64_t)num_seqs * num_kv_heads,
+                        record_rows(1, num_heads / num_kv_heads), head_size);
 }
 
 int tq4_kv8_paged_decode(void* stream, int element_type, int code_type, const void* q,
@@ -254,13 +272,14 @@ int tq4_kv8_paged_decode(void* stream, int element_type, int code_type, const vo
                           block_size, max_blocks_per_seq);
     if (rc != TQ4_OK) return rc;
     if (num_splits > TQ4_KV8_MAX_SPLITS) return TQ4_ERR_SPLITS;
-    const Splits s = split_rule((uint64_t)num_seqs * num_kv_heads,
-                                (uint64_t)max_blocks_per_seq * block_size, num_splits);
-    const size_t need = record_bytes(num_seqs, num_heads, head_size, s.K);
+    const uint64_t cap = (uint64_t)max_blocks_per_seq * block_size;
+    const Cut s = cut_rule(head_size, num_seqs, num_kv_heads, 1, cap, num_splits);
+    if (!cut_fits(s, num_seqs, cap, num_kv_heads, 1) || mul(num_seqs, num_heads) > kMaxGroups)
+        return TQ4_ERR_RANGE;
+    const size_t need = tq4_kv8_decode_workspace_bytes(num_seqs, num_heads, num_kv_heads, head_size,
+                                                       block_size, max_blocks_per_seq, num_splits);
     if (need && (!workspace || !aligned(workspace) || workspace_bytes < need))
         return TQ4_ERR_WORKSPACE;
-    if (mul(num_seqs, s.K) > kMaxGroups || mul(num_seqs, num_heads) > kMaxWaves)
-        return TQ4_ERR_RANGE;
     return launched(tq4::launch_kv8_decode(
         (hipStream_t)stream, element_type, code_type == TQ4_KV8_INT8,
         make(q, key_cache, value_cache, scale_cache, block_tables, context_lens, nullptr, out,
@@ -275,10 +294,11 @@ size_t tq4_kv8_prefill_workspace_bytes(uint32_t num_rows, uint32_t num_seqs, uin
 {
     if (num_kv_heads == 0) return 0;
     if (max_query_len > num_rows) max_query_len = num_rows;
-    const uint64_t tiles = tiles_of(max_query_len, num_heads / num_kv_heads);
-    const Splits s = split_rule((uint64_t)num_seqs * num_kv_heads * tiles,
-                                (uint64_t)max_blocks_per_seq * block_size, 0);
-    return record_bytes(num_rows, num_heads, head_size, s.K);
+    const uint64_t group = num_heads / num_kv_heads;
+    const Cut c = cut_rule(head_size, num_seqs, num_kv_heads, tiles_of(max_query_len, group),
+                           (uint64_t)max_blocks_per_seq * block_size, 0);
+    return record_bytes(c, mul(num_seqs, num_kv_heads, tiles_of(max_query_len, group)),
+                        record_rows(max_query_len, group), head_size);
 }
 
 int tq4_kv8_paged_prefill(void* stream, int element_type, int code_type, const void* q,
@@ -301,14 +321,15 @@ int tq4_kv8_paged_prefill(void* stream, int element_type, int code_type, const v
     if (!cu_seqlens) return TQ4_ERR_NULL_POINTER;
     if (max_query_len > num_rows) max_query_len = num_rows;
     const uint64_t tiles = tiles_of(max_query_len, num_heads / num_kv_heads);
-    const Splits s = split_rule((uint64_t)num_seqs * num_kv_heads * tiles,
-                                (uint64_t)max_blocks_per_seq * block_size, 0);
-    const size_t need = record_bytes(num_rows, num_heads, head_size, s.K);
+    const uint64_t cap = (uint64_t)max_blocks_per_seq * block_size;
+    const Cut s = cut_rule(head_size, num_seqs, num_kv_heads, tiles, cap, 0);
+    if (!cut_fits(s, num_seqs, cap, num_kv_heads, tiles) || mul(num_rows, num_heads) > kMaxGroups)
+        return TQ4_ERR_RANGE;
+    const size_t need =
+        tq4_kv8_prefill_workspace_bytes(num_rows, num_seqs, num_heads, num_kv_heads, head_size,
+                                        block_size, max_blocks_per_seq, max_query_len);
     if (need && (!workspace || !aligned(workspace) || workspace_bytes < need))
         return TQ4_ERR_WORKSPACE;
-    if (mul(num_seqs, s.K) > kMaxGroups || mul(num_rows, num_heads) > kMaxWaves ||
-        mul(num_kv_heads, tiles) > 65535u)
-        return TQ4_ERR_RANGE;
     return launched(tq4::launch_kv8_decode(
         (hipStream_t)stream, element_type, code_type == TQ4_KV8_INT8,
         make(q, key_cache, value_cache, scale_cache, block_tables, context_lens, cu_seqlens, out,

@@ -88,14 +88,30 @@ inline Divisor div_magic(uint32_t d)
     return {d == 1 ? 0x80000000u : (uint32_t)((1ull << shift) / d + 1), shift};
 }
 
-// The tokens that a split of a sequence of L tokens holds (a multiple of 64):
-// L cut into kmin parts, none longer than wmax.
-__device__ __forceinline__ uint32_t split_width(uint32_t L, uint32_t kmin, uint32_t wmin,
-                                                uint32_t wmax)
+// A lane's value from `CTRL`'s lane, 0 where there is none (or the row is masked).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v)
 {
-    uint32_t w = ((L + kmin - 1) / kmin + 63u) & ~63u;
-    if (w < wmin) w = wmin;
-    return w < wmax ? w : wmax;
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t moved(uint64_t v)
+{
+    return (uint64_t)moved<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | moved<CTRL, ROWS>((uint32_t)v);
+}
+
+// Inclusive sum over the wave: within rows of 16 lanes by shifts, then the rows'
+// last lanes to the rows behind them.
+template <class T>
+__device__ __forceinline__ T wave_scan(T v)
+{
+    v += moved<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);  // row_bcast:15 to rows 1 and 3
+    v += moved<0x143, 0xc>(v);  // row_bcast:31 to rows 2 and 3
+    return v;
 }
 
 // All 16 bytes of a strip's channel with those of dead tokens (>= live) zero.

@@ -31,18 +31,23 @@ struct Kv8WriteParams {
 };
 hipError_t launch_kv8_writer(hipStream_t stream, int bf16, int int8, const Kv8WriteParams& p);
 
-// Attention. Split k of a sequence of L tokens holds tokens [k*W, (k+1)*W), W
-// = split_width(L, ..) (kv8_device.hpp); cu NULL: one row a sequence.
+// Attention; cu NULL: one row a sequence.
+constexpr uint32_t kKv8Unit = 64, kKv8Rows = 16;  // tokens of a step, rows of a tile
+// Workgroups of the decode that a CU holds at once, by registers.
+constexpr int kKv8GroupsPerCu(int d) { return d == 256 ? 1 : d == 128 ? 2 : 4; }
+
 struct Kv8AttnParams {
     const void* q;
     const uint8_t *key_cache, *value_cache;
     const float* scales;
     const int32_t *tables, *context_lens, *cu;
-    float *acc, *ml;  // records: [row][K][D] and [row][K][2], row = q row * Hq + head
+    float *acc, *ml;  // records: [slot][rec_rows][D] and [slot][rec_rows][2]
     void* out;
     uint64_t q_stride;
     uint32_t rows, B, Hq, Hkv, G, D, S, P, M;
-    uint32_t K, kmin, wmin, wmax;  // splits, see split_width
+    uint32_t K;              // parts of a sequence; 0: streamed over `groups`
+    uint32_t groups, least;  // workgroups, and units that one takes at least
+    uint32_t rec_rows;
     uint32_t max_q;
     int causal;
     float scale;

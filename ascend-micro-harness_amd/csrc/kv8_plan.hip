@@ -21,6 +21,7 @@ namespace {
 
 using kv8::div_by;
 using kv8::Divisor;
+using kv8::wave_scan;
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
@@ -58,28 +59,6 @@ struct Pages {
         return (uint32_t)(i < P ? i : i - P);
     }
 };
-
-// A lane's value from `CTRL`'s lane, 0 where there is none (or the row is masked).
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint64_t moved(uint64_t v)
-{
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
-    return (uint64_t)hi << 32 | lo;
-}
-
-// Inclusive sum over the wave: within rows of 16 lanes by shifts, then the rows'
-// last lanes to the rows behind them.
-__device__ __forceinline__ uint64_t wave_scan(uint64_t v)
-{
-    v += moved<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
-    v += moved<0x112, 0xf>(v);
-    v += moved<0x114, 0xf>(v);
-    v += moved<0x118, 0xf>(v);
-    v += moved<0x142, 0xa>(v);  // row_bcast:15 to rows 1 and 3
-    v += moved<0x143, 0xc>(v);  // row_bcast:31 to rows 2 and 3
-    return v;
-}
 
 // Inclusive sum over the workgroup; `total` the whole. part: kWaves words of LDS
 // that nothing else uses up to the next barrier.
