@@ -88,6 +88,10 @@ size_t record_bytes(const Cut& c, uint64_t items, uint32_t rec_rows, uint32_t d)
     return b > (uint64_t)SIZE_MAX - 16 ? SIZE_MAX : (size_t)((b + 15) & ~15ull);
 }
 
+// Whether the decode kernel takes a prefill call: row tiles of 16 that each read
+// the context, split over it, against tiles of 128 and more in LDS.
+bool few_rows(uint64_t rows) { return rows <= 64; }
+
 // The grid and the line of a streamed call's units in bounds.
 bool cut_fits(const Cut& c, uint64_t seqs, uint64_t cap, uint64_t heads, uint64_t tiles)
 {
@@ -295,6 +299,7 @@ size_t tq4_kv8_prefill_workspace_bytes(uint32_t num_rows, uint32_t num_seqs, uin
     if (num_kv_heads == 0) return 0;
     if (max_query_len > num_rows) max_query_len = num_rows;
     const uint64_t group = num_heads / num_kv_heads;
+    if (!few_rows(max_query_len * group)) return 0;
     const Cut c = cut_rule(head_size, num_seqs, num_kv_heads, tiles_of(max_query_len, group),
                            (uint64_t)max_blocks_per_seq * block_size, 0);
     return record_bytes(c, mul(num_seqs, num_kv_heads, tiles_of(max_query_len, group)),
@@ -320,8 +325,19 @@ int tq4_kv8_paged_prefill(void* stream, int element_type, int code_type, const v
     if (rc != TQ4_OK) return rc;
     if (!cu_seqlens) return TQ4_ERR_NULL_POINTER;
     if (max_query_len > num_rows) max_query_len = num_rows;
-    const uint64_t tiles = tiles_of(max_query_len, num_heads / num_kv_heads);
-    const uint64_t cap = (uint64_t)max_blocks_per_seq * block_size;
+    const uint64_t group = num_heads / num_kv_heads, tiles = tiles_of(max_query_len, group);
+    const uint64_t cap = (uint64_t)max_blocks_per_seq * block_size, rows = (uint64_t)num_rows * group;
+    auto args = [&](const Cut& c) {
+        return make(q, key_cache, value_cache, scale_cache, block_tables, context_lens, cu_seqlens,
+                    out, q_stride, num_rows, num_seqs, num_heads, num_kv_heads, head_size,
+                    block_size, num_blocks, max_blocks_per_seq, max_query_len, causal != 0, scale,
+                    c, workspace);
+    };
+    if (!few_rows(max_query_len * group)) {
+        if (mul(rows / 128 + num_seqs, num_kv_heads) > kMaxGroups) return TQ4_ERR_RANGE;
+        return launched(tq4::launch_kv8_prefill((hipStream_t)stream, element_type,
+                                                code_type == TQ4_KV8_INT8, args(Cut{1, 0, 0})));
+    }
     const Cut s = cut_rule(head_size, num_seqs, num_kv_heads, tiles, cap, 0);
     if (!cut_fits(s, num_seqs, cap, num_kv_heads, tiles) || mul(num_rows, num_heads) > kMaxGroups)
         return TQ4_ERR_RANGE;
@@ -330,11 +346,8 @@ int tq4_kv8_paged_prefill(void* stream, int element_type, int code_type, const v
                                         block_size, max_blocks_per_seq, max_query_len);
     if (need && (!workspace || !aligned(workspace) || workspace_bytes < need))
         return TQ4_ERR_WORKSPACE;
-    return launched(tq4::launch_kv8_decode(
-        (hipStream_t)stream, element_type, code_type == TQ4_KV8_INT8,
-        make(q, key_cache, value_cache, scale_cache, block_tables, context_lens, cu_seqlens, out,
-             q_stride, num_rows, num_seqs, num_heads, num_kv_heads, head_size, block_size,
-             num_blocks, max_blocks_per_seq, max_query_len, causal != 0, scale, s, workspace)));
+    return launched(tq4::launch_kv8_decode((hipStream_t)stream, element_type,
+                                           code_type == TQ4_KV8_INT8, args(s)));
 }
 
 }  // extern "C"

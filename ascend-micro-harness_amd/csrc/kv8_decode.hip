@@ -113,25 +113,9 @@ struct ValueBytes {
     }
 };
 
-// A sequence's rows and tokens, held in bounds.
-struct Sequence {
-    uint32_t row0, rows, all, tokens;  // rows: those computed, of all
-
+struct Sequence : SequenceBase {
     __device__ __forceinline__ Sequence() {}
-    __device__ __forceinline__ Sequence(const Kv8AttnParams& p, uint32_t b)
-    {
-        row0 = b;
-        all = 1;
-        if (p.cu) {
-            const int32_t from = p.cu[b], to = p.cu[b + 1];
-            row0 = (uint32_t)from;
-            all = from >= 0 && to > from ? (uint32_t)(to - from) : 0u;
-        }
-        rows = all < p.max_q ? all : p.max_q;
-        const int32_t len = p.context_lens[b];
-        const uint32_t cap = p.M * p.S;  // below 2^31
-        tokens = len < 0 ? 0u : (uint32_t)len < cap ? (uint32_t)len : cap;
-    }
+    __device__ __forceinline__ Sequence(const Kv8AttnParams& p, uint32_t b) : SequenceBase(p, b) {}
     // An item is a (sequence, kv head, tile of 16 rows); its units of 64 tokens:
     // one at least, which writes the zeros of rows that see nothing.
     __device__ __forceinline__ uint32_t units() const
@@ -149,10 +133,7 @@ struct Sequence {
     __device__ __forceinline__ Sequence of_lane(uint32_t lane) const
     {
         Sequence s;
-        s.row0 = __builtin_amdgcn_readlane(row0, lane);
-        s.rows = __builtin_amdgcn_readlane(rows, lane);
-        s.all = __builtin_amdgcn_readlane(all, lane);
-        s.tokens = __builtin_amdgcn_readlane(tokens, lane);
+        static_cast<SequenceBase&>(s) = SequenceBase::of_lane(lane);
         return s;
     }
 };

@@ -126,5 +126,35 @@ __device__ __forceinline__ u4_t live_bytes(u4_t v, int live)
     return v;
 }
 
+// A sequence's rows and tokens, held in bounds.
+struct SequenceBase {
+    uint32_t row0, rows, all, tokens;  // rows: those computed, of all
+
+    __device__ __forceinline__ SequenceBase() {}
+    __device__ __forceinline__ SequenceBase(const Kv8AttnParams& p, uint32_t b)
+    {
+        row0 = b;
+        all = 1;
+        if (p.cu) {
+            const int32_t from = p.cu[b], to = p.cu[b + 1];
+            row0 = (uint32_t)from;
+            all = from >= 0 && to > from ? (uint32_t)(to - from) : 0u;
+        }
+        rows = all < p.max_q ? all : p.max_q;
+        const int32_t len = p.context_lens[b];
+        const uint32_t cap = p.M * p.S;  // below 2^31
+        tokens = len < 0 ? 0u : (uint32_t)len < cap ? (uint32_t)len : cap;
+    }
+    __device__ __forceinline__ SequenceBase of_lane(uint32_t lane) const
+    {
+        SequenceBase s;
+        s.row0 = __builtin_amdgcn_readlane(row0, lane);
+        s.rows = __builtin_amdgcn_readlane(rows, lane);
+        s.all = __builtin_amdgcn_readlane(all, lane);
+        s.tokens = __builtin_amdgcn_readlane(tokens, lane);
+        return s;
+    }
+};
+
 }  // namespace kv8
 }  // namespace tq4

@@ -1,0 +1,410 @@
+// kv8_prefill.hip -- attention of many rows a sequence over the 8-bit paged cache
+// (tq4_kv8_paged_prefill of prompt chunks and cross attention; tq4_kv8.h).
+//
+// A workgroup takes 128 * RB rows of a (sequence, kv head): query tokens times the
+// GQA group's heads, so the group shares each key. A wave has 32 * RB of them and
+// walks the tokens 64 at a time with its workgroup:
+//   S = K Q^T       MFMA 32x32x16 f16, 32 tokens x 32 rows
+//   s' = S * (k scale * q factor) + log2(v scale)
+//   P = 2^(s' - m)  in f16, the v scale inside it (kv8_decode.hip)
+//   O^T += V^T P^T, l += P / v scale, out = O / l
+// The tile's codes are widened to f16 once, on their way into LDS, in the order in
+// which the matrix operands are read (a lane's 16 bytes next to its neighbour's).
+// Tokens are permuted inside a block of 32 so that a lane's scores are, as they
+// lie, the P^T operand of 8 consecutive tokens of a strip, half a value row: row
+// m = 16 s + 8 a + 4 half + i of the block is token 16 s + 8 half + 4 a + i.
+// Two LDS buffers: tile j is computed while tile j + 1 is widened into the other
+// and tile j + 2 comes from memory.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "kv8_device.hpp"
+
+namespace tq4 {
+namespace {
+
+using namespace kv8;
+
+typedef float f16_t __attribute__((ext_vector_type(16)));
+
+constexpr int kThreads = 256;
+constexpr int kTile = 64;             // tokens
+constexpr int kStrips = kTile / 16;
+
+// Rows in a workgroup.
+constexpr uint32_t group_rows(int rb) { return 128u * rb; }
+
+// LDS of a tile: operand blocks of 64 lanes x 16 bytes. Keys: [block of 32
+// tokens][16 channels]; values: [strip][32 channels]. Key blocks lie 16 bytes
+// further apart than their size, which spreads a wave's stores over the banks.
+template <int D>
+struct Tile {
+    static constexpr int kKeyBlock = 1024 + 16;
+    static constexpr int kKeys = 2 * (D / 16) * kKeyBlock;
+    static constexpr int kValues = kStrips * (D / 32) * 1024;
+    static constexpr int kBytes = kKeys + kValues;
+};
+
+struct StripInfo {
+    float ks, lv, rvs;  // key scale, log2 and reciprocal of the value scale
+    int live;           // its live tokens
+};
+
+// What a thread brings of a tile: D / 64 pieces of 16 bytes of each plane. Key
+// piece u: token u / (D / 16), channels 16 * (u % (D / 16)) ..; value piece u:
+// strip u / D, channel u % D.
+template <int D, int INT8>
+struct Stage {
+    static constexpr int N = D / 64;
+    u4_t k[N], v[N];
+    int live[N];      // live tokens of the value pieces' strips
+    int32_t e[N], es;  // the next fetch's block-table entries, -1: no page
+    float ks, vs;      // of strip threadIdx.x, its live tokens
+    int own;
+
+    static __device__ __forceinline__ uint32_t piece(int r) { return r * kThreads + threadIdx.x; }
+
+    __device__ __forceinline__ int32_t entry(const Kv8AttnParams& p, const int32_t* table,
+                                             Divisor per_page, uint32_t strip) const
+    {
+        const uint32_t i = div_by(strip, per_page);
+        const int32_t e = table[i < p.M ? i : p.M - 1];
+        return i < p.M && e >= 0 && (uint32_t)e < p.P ? e : -1;
+    }
+    __device__ __forceinline__ void entries(const Kv8AttnParams& p, const int32_t* table,
+                                            Divisor per_page, uint32_t t0)
+    {
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+            // both planes' pieces u lie in strip u / D of the tile
+            e[r] = entry(p, table, per_page, t0 / 16 + piece(r) / D);
+        }
+        es = entry(p, table, per_page, t0 / 16 + (threadIdx.x & 3u));
+    }
+    __device__ __forceinline__ void fetch(const Kv8AttnParams& p, Divisor per_page, uint32_t h,
+                                          uint32_t L, uint32_t t0)
+    {
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+            const uint32_t u = piece(r);
+            const uint32_t strip = t0 / 16 + u / D;
+            const uint32_t in = strip - div_by(strip, per_page) * (p.S / 16);
+            const uint64_t row = (uint64_t)(uint32_t)(e[r] < 0 ? 0 : e[r]) * p.Hkv + h;
+            const uint32_t token = u / (D / 16) % 16;
+            k[r] = *(const u4_t*)(p.key_cache + (row * p.S + in * 16 + token) * D +
+                                  16 * (u % (D / 16)));
+            v[r] = *(const u4_t*)(p.value_cache + (row * p.S + in * 16) * D + 16 * (u % D));
+            const int left = (int)L - (int)(16 * strip);
+            live[r] = e[r] < 0 || left < 0 ? 0 : left > 16 ? 16 : left;
+        }
+        const uint64_t row = (uint64_t)(uint32_t)(es < 0 ? 0 : es) * p.Hkv + h;
+        ks = p.scales[row];
+        vs = p.scales[(uint64_t)p.P * p.Hkv + row];
+        const int left = (int)L - (int)(t0 + 16 * (threadIdx.x & 3u));
+        own = es < 0 || left < 0 ? 0 : left > 16 ? 16 : left;
+    }
+    __device__ __forceinline__ void store(char* tile, StripInfo* info) const
+    {
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+            const uint32_t u = piece(r);
+            {
+                const uint32_t token = u / (D / 16), block = token / 32, x = token % 32;
+                const uint32_t m = (x & 16) | (x & 4) << 1 | (x & 8) >> 1 | (x & 3);
+                char* to = tile + (block * (D / 16) + u % (D / 16)) * Tile<D>::kKeyBlock + m * 16;
+                *(h8_t*)to = widen8<INT8>(k[r][0], k[r][1]);
+                *(h8_t*)(to + 512) = widen8<INT8>(k[r][2], k[r][3]);
+            }
+            {
+                // a dead token's bytes may be a NaN: 0 times it is not 0
+                const u4_t w = live[r] < 16 ? live_bytes(v[r], live[r]) : v[r];
+                const uint32_t strip = u / D, c = u % D;
+                char* to = tile + Tile<D>::kKeys + (strip * (D / 32) + c / 32) * 1024 + (c % 32) * 16;
+                *(h8_t*)to = widen8<INT8>(w[0], w[1]);
+                *(h8_t*)(to + 512) = widen8<INT8>(w[2], w[3]);
+            }
+        }
+        if (threadIdx.x < kStrips) {
+            const float s = held_scale(vs);
+            StripInfo i;
+            i.ks = held_scale(ks);
+            i.lv = __builtin_amdgcn_logf(s);
+            i.rvs = __builtin_amdgcn_rcpf(s);
+            i.live = own;
+            info[threadIdx.x] = i;
+        }
+    }
+};
+
+template <int D, int BF16, int INT8, int RB>
+__global__ __launch_bounds__(kThreads, 1) void kv8_prefill(Kv8AttnParams p, Divisor per_page)
+{
+    constexpr int KK = D / 16, CB = D / 32;
+    __shared__ __align__(16) char lds[2 * Tile<D>::kBytes];
+    __shared__ StripInfo info[2][kStrips];
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
+    const uint32_t n = lane & 31u, half = lane >> 5;
+
+    // the heads of a tile lie next to each other in the grid (one an XCD, where
+    // there are eight); a sequence's last tiles, the longest, come first
+    const uint32_t h = blockIdx.x % p.Hkv;
+    uint32_t t = gridDim.x / p.Hkv - 1 - blockIdx.x / p.Hkv, b = 0;
+    SequenceBase seq;
+    {
+        uint32_t before = 0;
+        for (uint32_t b0 = 0;; b0 += 64) {
+            if (b0 >= p.B) return;
+            uint32_t tiles = 0;
+            SequenceBase mine;
+            if (b0 + lane < p.B) {
+                mine = SequenceBase(p, b0 + lane);
+                tiles = (mine.rows * p.G + group_rows(RB) - 1) / group_rows(RB);
+            }
+            const uint32_t upto = before + wave_scan(tiles);
+            const uint64_t past = __ballot(upto > t);
+            if (past) {
+                const uint32_t l = (uint32_t)__builtin_ctzll(past);
+                b = b0 + l;
+                seq = mine.of_lane(l);
+                t -= __builtin_amdgcn_readlane(upto - tiles, l);
+                break;
+            }
+            before = __builtin_amdgcn_readlane(upto, 63);
+        }
+    }
+    const uint32_t f0 = t * group_rows(RB), all_rows = seq.rows * p.G;
+    const int32_t* table = p.tables + (uint64_t)b * p.M;
+
+    // the lane's rows, and the tokens before `limit` that each sees
+    h8_t q[RB][KK];
+    float qf[RB], m[RB], l[RB];
+    int32_t limit[RB];
+    f16_t o[RB][CB];
+    const float scale = fabsf(p.scale) * kLog2e;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const uint32_t f = f0 + (wave * RB + rb) * 32 + n;
+        const uint32_t fr = f < all_rows ? f : all_rows - 1;
+        uint32_t row = seq.row0 + fr / p.G;
+        if (row >= p.rows) row = p.rows - 1;
+        limit[rb] = (int32_t)seq.tokens;
+        if (p.causal) {
+            const int64_t x = (int64_t)seq.tokens - seq.all + fr / p.G + 1;
+            limit[rb] = x < 0 ? 0 : (int32_t)x;
+        }
+        const uint16_t* src = (const uint16_t*)p.q + (uint64_t)row * p.q_stride +
+                              (uint64_t)(h * p.G + fr % p.G) * D + 8 * half;
+        u4_t raw[KK];
+#pragma unroll
+        for (int k = 0; k < KK; ++k) raw[k] = *(const u4_t*)(src + 16 * k);
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KK * 8; ++i) {
+            const uint32_t w = raw[i / 8][(i / 2) & 3];
+            most = fmaxf(most, fabsf(widen_el<BF16>((i & 1) ? w >> 16 : w & 0xffffu)));
+        }
+        most = fmaxf(most, xor_lanes(most, 32));
+        const float shift = row_shift(most);
+        qf[rb] = (1.0f / shift) * scale;
+        // a negative scale turns the row, so that larger products are larger scores
+        const float turned = p.scale < 0.0f ? -shift : shift;
+#pragma unroll
+        for (int i = 0; i < KK * 8; ++i) {
+            const uint32_t w = raw[i / 8][(i / 2) & 3];
+            q[rb][i / 8][i % 8] =
+                (_Float16)(widen_el<BF16>((i & 1) ? w >> 16 : w & 0xffffu) * turned);
+        }
+        m[rb] = kNone;
+        l[rb] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[rb][c][i] = 0.0f;
+    }
+
+    // tokens that the workgroup's rows see, and that every row of the wave sees
+    const uint32_t last = f0 + group_rows(RB) < all_rows ? f0 + group_rows(RB) - 1 : all_rows - 1;
+    uint32_t end = seq.tokens;
+    int32_t whole = (int32_t)seq.tokens, some = (int32_t)seq.tokens;
+    if (p.causal) {
+        const int64_t x = (int64_t)seq.tokens - seq.all + last / p.G + 1;
+        end = x < 0 ? 0u : (uint32_t)x;
+        const uint32_t wf = f0 + wave * 32 * RB;
+        const int64_t y = (int64_t)seq.tokens - seq.all + wf / p.G + 1;
+        whole = y < 0 ? 0 : y < seq.tokens ? (int32_t)y : (int32_t)seq.tokens;
+        const int64_t z = (int64_t)seq.tokens - seq.all + (wf + 32 * RB - 1) / p.G + 1;
+        some = z < 0 ? 0 : z < seq.tokens ? (int32_t)z : (int32_t)seq.tokens;
+    }
+    if (f0 + wave * 32 * RB >= all_rows) some = 0;  // no row of its own
+    const uint32_t tiles = (end + kTile - 1) / kTile;
+
+    Stage<D, INT8> stage;
+    if (tiles) {
+        stage.entries(p, table, per_page, 0);
+        stage.fetch(p, per_page, h, seq.tokens, 0);
+        stage.store(lds, info[0]);
+    }
+    if (tiles > 1) {
+        stage.entries(p, table, per_page, kTile);
+        stage.fetch(p, per_page, h, seq.tokens, kTile);
+        stage.entries(p, table, per_page, 2 * kTile);
+    }
+    for (uint32_t j = 0; j < tiles; ++j) {
+        __syncthreads();  // tile j is in LDS, the other buffer has been read
+        char* tile = lds + (j & 1) * Tile<D>::kBytes;
+        const StripInfo* at = info[j & 1];
+        const int32_t t0 = (int32_t)(j * kTile);
+        if (j + 1 < tiles) {
+            stage.store(lds + ((j + 1) & 1) * Tile<D>::kBytes, info[(j + 1) & 1]);
+            if (j + 2 < tiles) {
+                // (the entries of tile j + 2 came a tile ago)
+                stage.fetch(p, per_page, h, seq.tokens, t0 + 2 * kTile);
+                stage.entries(p, table, per_page, t0 + 3 * kTile);
+            }
+        }
+        if (t0 >= some) continue;
+
+        f16_t s[2][RB];
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[tb][rb][i] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KK; ++k) {
+                const h8_t a = *(const h8_t*)(tile + (tb * KK + k) * Tile<D>::kKeyBlock + lane * 16);
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+                    s[tb][rb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[rb][k], s[tb][rb], 0, 0, 0);
+            }
+        }
+        StripInfo st[kStrips];
+        int least = 16;
+#pragma unroll
+        for (int i = 0; i < kStrips; ++i) {
+            st[i] = at[i];
+            least = st[i].live < least ? st[i].live : least;
+        }
+        if (least < 16 || t0 + kTile > whole) {
+            // token 8 half + 4 a + i of strip x
+#pragma unroll
+            for (int x = 0; x < kStrips; ++x)
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    const int ahead = limit[rb] - t0 - 16 * x;
+                    const int sees = ahead < st[x].live ? ahead : st[x].live;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float y = s[x / 2][rb][8 * (x & 1) + i];
+                        s[x / 2][rb][8 * (x & 1) + i] =
+                            (int)(8 * half) + i < sees ? y : -__builtin_inff();
+                    }
+                }
+        }
+        h8_t pr[RB][kStrips];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            float fac[kStrips], most = -__builtin_inff();
+#pragma unroll
+            for (int x = 0; x < kStrips; ++x) {
+                // (not 0: a masked score is -inf)
+                fac[x] = fmaxf(st[x].ks * qf[rb], 1e-37f);
+                float y = s[x / 2][rb][8 * (x & 1)];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) y = fmaxf(y, s[x / 2][rb][8 * (x & 1) + i]);
+                most = fmaxf(most, __builtin_fmaf(y, fac[x], st[x].lv));
+            }
+            if (__any(most > m[rb] + 14.0f)) {
+                most = fmaxf(most, xor_lanes(most, 32));
+                const float to = fmaxf(m[rb], most - 6.0f);
+                const float r = __builtin_amdgcn_exp2f(m[rb] - to);
+                m[rb] = to;
+                l[rb] *= r;
+#pragma unroll
+                for (int c = 0; c < CB; ++c) o[rb][c] *= r;
+            }
+#pragma unroll
+            for (int x = 0; x < kStrips; ++x) {
+                const float off = st[x].lv - m[rb];
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(
+                        __builtin_fmaf(s[x / 2][rb][8 * (x & 1) + i], fac[x], off));
+                    sum += e;
+                    pr[rb][x][i] = (_Float16)e;
+                }
+                l[rb] += sum * st[x].rvs;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+            for (int x = 0; x < kStrips; ++x) {
+                const h8_t a =
+                    *(const h8_t*)(tile + Tile<D>::kKeys + (x * CB + c) * 1024 + lane * 16);
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+                    o[rb][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pr[rb][x], o[rb][c], 0, 0, 0);
+            }
+    }
+
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const uint32_t f = f0 + (wave * RB + rb) * 32 + n, row = seq.row0 + f / p.G;
+        const float sum = l[rb] + xor_lanes(l[rb], 32);
+        if (f >= all_rows || row >= p.rows) continue;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        uint16_t* out = (uint16_t*)p.out + ((uint64_t)row * p.Hq + h * p.G + f % p.G) * D + 4 * half;
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                *(u2_t*)(out + 32 * c + 8 * x) =
+                    u2_t{narrow2<BF16>(o[rb][c][4 * x] * inv, o[rb][c][4 * x + 1] * inv),
+                         narrow2<BF16>(o[rb][c][4 * x + 2] * inv, o[rb][c][4 * x + 3] * inv)};
+    }
+}
+
+template <int D, int BF16, int INT8, int RB>
+hipError_t launch_t(hipStream_t stream, const Kv8AttnParams& p)
+{
+    // at most so many tiles: whole ones of all rows, and one more a sequence
+    const uint64_t rows = (uint64_t)p.rows * p.G;
+    const uint64_t tiles = rows / group_rows(RB) + (p.B < rows ? p.B : rows);
+    hipLaunchKernelGGL((kv8_prefill<D, BF16, INT8, RB>), dim3((uint32_t)(tiles * p.Hkv)),
+                       dim3(kThreads), 0, stream, p, div_magic(p.S / 16));
+    return hipGetLastError();
+}
+
+template <int D, int BF16, int INT8>
+hipError_t launch_rb(hipStream_t stream, const Kv8AttnParams& p)
+{
+    // 64 rows of 256 channels and their sums pass a wave's registers
+    if constexpr (D < 256) {
+        if (p.max_q * p.G > 128) return launch_t<D, BF16, INT8, 2>(stream, p);
+    }
+    return launch_t<D, BF16, INT8, 1>(stream, p);
+}
+
+template <int D>
+hipError_t launch_d(hipStream_t stream, int bf16, int int8, const Kv8AttnParams& p)
+{
+    if (bf16) return int8 ? launch_rb<D, 1, 1>(stream, p) : launch_rb<D, 1, 0>(stream, p);
+    return int8 ? launch_rb<D, 0, 1>(stream, p) : launch_rb<D, 0, 0>(stream, p);
+}
+
+}  // namespace
+
+hipError_t launch_kv8_prefill(hipStream_t stream, int bf16, int int8, const Kv8AttnParams& p)
+{
+    switch (p.D) {
+        case 64: return launch_d<64>(stream, bf16, int8, p);
+        case 128: return launch_d<128>(stream, bf16, int8, p);
+        case 256: return launch_d<256>(stream, bf16, int8, p);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace tq4
