@@ -1,8 +1,8 @@
 // kv8_prefill.hip -- attention of many rows a sequence over the 8-bit paged cache
 // (tq4_kv8_paged_prefill of prompt chunks and cross attention; tq4_kv8.h).
 //
-// A workgroup takes 128 * RB rows of a (sequence, kv head): query tokens times the
-// GQA group's heads, so the group shares each key. A wave has 32 * RB of them and
+// A workgroup takes 256 (or 128) rows of a (sequence, kv head): query tokens times
+// the GQA group's heads, so the group shares each key. A wave has 32 of them and
 // walks the tokens 64 at a time with its workgroup:
 //   S = K Q^T       MFMA 32x32x16 f16, 32 tokens x 32 rows
 //   s' = S * (k scale * q factor) + log2(v scale)
@@ -27,12 +27,11 @@ using namespace kv8;
 
 typedef float f16_t __attribute__((ext_vector_type(16)));
 
-constexpr int kThreads = 256;
 constexpr int kTile = 64;             // tokens
 constexpr int kStrips = kTile / 16;
 
-// Rows in a workgroup.
-constexpr uint32_t group_rows(int rb) { return 128u * rb; }
+// Rows of a workgroup of W waves.
+constexpr uint32_t group_rows(int w) { return 32u * w; }
 
 // LDS of a tile: operand blocks of 64 lanes x 16 bytes. Keys: [block of 32
 // tokens][16 channels]; values: [strip][32 channels]. Key blocks lie 16 bytes
@@ -50,19 +49,24 @@ struct StripInfo {
     int live;           // its live tokens
 };
 
-// What a thread brings of a tile: D / 64 pieces of 16 bytes of each plane. Key
+// What a thread brings of a tile: N pieces of 16 bytes of each plane, of 4 * D. Key
 // piece u: token u / (D / 16), channels 16 * (u % (D / 16)) ..; value piece u:
 // strip u / D, channel u % D.
-template <int D, int INT8>
+template <int D, int INT8, int W>
 struct Stage {
-    static constexpr int N = D / 64;
+    static constexpr int kThreads = 64 * W, kPieces = 4 * D;
+    static constexpr int N = (kPieces + kThreads - 1) / kThreads;
     u4_t k[N], v[N];
     int live[N];      // live tokens of the value pieces' strips
     int32_t e[N], es;  // the next fetch's block-table entries, -1: no page
     float ks, vs;      // of strip threadIdx.x, its live tokens
     int own;
 
-    static __device__ __forceinline__ uint32_t piece(int r) { return r * kThreads + threadIdx.x; }
+    // (a thread too many brings another's piece, and does not store it)
+    static __device__ __forceinline__ uint32_t piece(int r)
+    {
+        return (r * kThreads + threadIdx.x) % kPieces;
+    }
 
     __device__ __forceinline__ int32_t entry(const Kv8AttnParams& p, const int32_t* table,
                                              Divisor per_page, uint32_t strip) const
@@ -107,6 +111,7 @@ struct Stage {
     {
 #pragma unroll
         for (int r = 0; r < N; ++r) {
+            if (N * kThreads > kPieces && r * kThreads + threadIdx.x >= kPieces) break;
             const uint32_t u = piece(r);
             {
                 const uint32_t token = u / (D / 16), block = token / 32, x = token % 32;
@@ -136,8 +141,9 @@ struct Stage {
     }
 };
 
-template <int D, int BF16, int INT8, int RB>
-__global__ __launch_bounds__(kThreads, 1) void kv8_prefill(Kv8AttnParams p, Divisor per_page)
+template <int D, int BF16, int INT8, int W>
+__global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnParams p,
+                                                                       Divisor per_page)
 {
     constexpr int KK = D / 16, CB = D / 32;
     __shared__ __align__(16) char lds[2 * Tile<D>::kBytes];
@@ -158,7 +164,7 @@ __global__ __launch_bounds__(kThreads, 1) void kv8_prefill(Kv8AttnParams p, Divi
             SequenceBase mine;
             if (b0 + lane < p.B) {
                 mine = SequenceBase(p, b0 + lane);
-                tiles = (mine.rows * p.G + group_rows(RB) - 1) / group_rows(RB);
+                tiles = (mine.rows * p.G + group_rows(W) - 1) / group_rows(W);
             }
             const uint32_t upto = before + wave_scan(tiles);
             const uint64_t past = __ballot(upto > t);
@@ -172,26 +178,22 @@ __global__ __launch_bounds__(kThreads, 1) void kv8_prefill(Kv8AttnParams p, Divi
             before = __builtin_amdgcn_readlane(upto, 63);
         }
     }
-    const uint32_t f0 = t * group_rows(RB), all_rows = seq.rows * p.G;
+    const uint32_t f0 = t * group_rows(W), all_rows = seq.rows * p.G;
     const int32_t* table = p.tables + (uint64_t)b * p.M;
 
-    // the lane's rows, and the tokens before `limit` that each sees
-    h8_t q[RB][KK];
-    float qf[RB], m[RB], l[RB];
-    int32_t limit[RB];
-    f16_t o[RB][CB];
-    const float scale = fabsf(p.scale) * kLog2e;
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        const uint32_t f = f0 + (wave * RB + rb) * 32 + n;
-        const uint32_t fr = f < all_rows ? f : all_rows - 1;
+    // the lane's row, and the tokens before `limit` that it sees
+    const uint32_t f = f0 + wave * 32 + n, fr = f < all_rows ? f : all_rows - 1;
+    int32_t limit = (int32_t)seq.tokens;
+    if (p.causal) {
+        const int64_t x = (int64_t)seq.tokens - seq.all + fr / p.G + 1;
+        limit = x < 0 ? 0 : (int32_t)x;
+    }
+    h8_t q[KK];
+    float qf, m = kNone, l = 0.0f;
+    f16_t o[CB];
+    {
         uint32_t row = seq.row0 + fr / p.G;
         if (row >= p.rows) row = p.rows - 1;
-        limit[rb] = (int32_t)seq.tokens;
-        if (p.causal) {
-            const int64_t x = (int64_t)seq.tokens - seq.all + fr / p.G + 1;
-            limit[rb] = x < 0 ? 0 : (int32_t)x;
-        }
         const uint16_t* src = (const uint16_t*)p.q + (uint64_t)row * p.q_stride +
                               (uint64_t)(h * p.G + fr % p.G) * D + 8 * half;
         u4_t raw[KK];
@@ -205,40 +207,37 @@ __global__ __launch_bounds__(kThreads, 1) void kv8_prefill(Kv8AttnParams p, Divi
         }
         most = fmaxf(most, xor_lanes(most, 32));
         const float shift = row_shift(most);
-        qf[rb] = (1.0f / shift) * scale;
+        qf = (1.0f / shift) * (fabsf(p.scale) * kLog2e);
         // a negative scale turns the row, so that larger products are larger scores
         const float turned = p.scale < 0.0f ? -shift : shift;
 #pragma unroll
         for (int i = 0; i < KK * 8; ++i) {
             const uint32_t w = raw[i / 8][(i / 2) & 3];
-            q[rb][i / 8][i % 8] =
-                (_Float16)(widen_el<BF16>((i & 1) ? w >> 16 : w & 0xffffu) * turned);
+            q[i / 8][i % 8] = (_Float16)(widen_el<BF16>((i & 1) ? w >> 16 : w & 0xffffu) * turned);
         }
-        m[rb] = kNone;
-        l[rb] = 0.0f;
 #pragma unroll
         for (int c = 0; c < CB; ++c)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[rb][c][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
     }
 
     // tokens that the workgroup's rows see, and that every row of the wave sees
-    const uint32_t last = f0 + group_rows(RB) < all_rows ? f0 + group_rows(RB) - 1 : all_rows - 1;
+    const uint32_t last = f0 + group_rows(W) < all_rows ? f0 + group_rows(W) - 1 : all_rows - 1;
     uint32_t end = seq.tokens;
     int32_t whole = (int32_t)seq.tokens, some = (int32_t)seq.tokens;
     if (p.causal) {
         const int64_t x = (int64_t)seq.tokens - seq.all + last / p.G + 1;
         end = x < 0 ? 0u : (uint32_t)x;
-        const uint32_t wf = f0 + wave * 32 * RB;
+        const uint32_t wf = f0 + wave * 32;
         const int64_t y = (int64_t)seq.tokens - seq.all + wf / p.G + 1;
         whole = y < 0 ? 0 : y < seq.tokens ? (int32_t)y : (int32_t)seq.tokens;
-        const int64_t z = (int64_t)seq.tokens - seq.all + (wf + 32 * RB - 1) / p.G + 1;
+        const int64_t z = (int64_t)seq.tokens - seq.all + (wf + 31) / p.G + 1;
         some = z < 0 ? 0 : z < seq.tokens ? (int32_t)z : (int32_t)seq.tokens;
     }
-    if (f0 + wave * 32 * RB >= all_rows) some = 0;  // no row of its own
+    if (f0 + wave * 32 >= all_rows) some = 0;  // no row of its own
     const uint32_t tiles = (end + kTile - 1) / kTile;
 
-    Stage<D, INT8> stage;
+    Stage<D, INT8, W> stage;
     if (tiles) {
         stage.entries(p, table, per_page, 0);
         stage.fetch(p, per_page, h, seq.tokens, 0);
@@ -264,135 +263,120 @@ __global__ __launch_bounds__(kThreads, 1) void kv8_prefill(Kv8AttnParams p, Divi
         }
         if (t0 >= some) continue;
 
-        f16_t s[2][RB];
+        f16_t s[2];
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb) {
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb)
+            for (int i = 0; i < 16; ++i) s[tb][i] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[tb][rb][i] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < KK; ++k) {
-                const h8_t a = *(const h8_t*)(tile + (tb * KK + k) * Tile<D>::kKeyBlock + lane * 16);
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
-                    s[tb][rb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[rb][k], s[tb][rb], 0, 0, 0);
-            }
+            for (int k = 0; k < KK; ++k)
+                s[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                    *(const h8_t*)(tile + (tb * KK + k) * Tile<D>::kKeyBlock + lane * 16), q[k],
+                    s[tb], 0, 0, 0);
         }
         StripInfo st[kStrips];
         int least = 16;
 #pragma unroll
-        for (int i = 0; i < kStrips; ++i) {
-            st[i] = at[i];
-            least = st[i].live < least ? st[i].live : least;
+        for (int x = 0; x < kStrips; ++x) {
+            st[x] = at[x];
+            least = st[x].live < least ? st[x].live : least;
         }
         if (least < 16 || t0 + kTile > whole) {
-            // token 8 half + 4 a + i of strip x
-#pragma unroll
-            for (int x = 0; x < kStrips; ++x)
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    const int ahead = limit[rb] - t0 - 16 * x;
-                    const int sees = ahead < st[x].live ? ahead : st[x].live;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float y = s[x / 2][rb][8 * (x & 1) + i];
-                        s[x / 2][rb][8 * (x & 1) + i] =
-                            (int)(8 * half) + i < sees ? y : -__builtin_inff();
-                    }
-                }
-        }
-        h8_t pr[RB][kStrips];
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            float fac[kStrips], most = -__builtin_inff();
+            // token 8 half + i of strip x
 #pragma unroll
             for (int x = 0; x < kStrips; ++x) {
-                // (not 0: a masked score is -inf)
-                fac[x] = fmaxf(st[x].ks * qf[rb], 1e-37f);
-                float y = s[x / 2][rb][8 * (x & 1)];
-#pragma unroll
-                for (int i = 1; i < 8; ++i) y = fmaxf(y, s[x / 2][rb][8 * (x & 1) + i]);
-                most = fmaxf(most, __builtin_fmaf(y, fac[x], st[x].lv));
-            }
-            if (__any(most > m[rb] + 14.0f)) {
-                most = fmaxf(most, xor_lanes(most, 32));
-                const float to = fmaxf(m[rb], most - 6.0f);
-                const float r = __builtin_amdgcn_exp2f(m[rb] - to);
-                m[rb] = to;
-                l[rb] *= r;
-#pragma unroll
-                for (int c = 0; c < CB; ++c) o[rb][c] *= r;
-            }
-#pragma unroll
-            for (int x = 0; x < kStrips; ++x) {
-                const float off = st[x].lv - m[rb];
-                float sum = 0.0f;
+                const int ahead = limit - t0 - 16 * x;
+                const int sees = (ahead < st[x].live ? ahead : st[x].live) - (int)(8 * half);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(
-                        __builtin_fmaf(s[x / 2][rb][8 * (x & 1) + i], fac[x], off));
-                    sum += e;
-                    pr[rb][x][i] = (_Float16)e;
+                    const float y = s[x / 2][8 * (x & 1) + i];
+                    s[x / 2][8 * (x & 1) + i] = i < sees ? y : -__builtin_inff();
                 }
-                l[rb] += sum * st[x].rvs;
             }
+        }
+        float fac[kStrips], most = -__builtin_inff();
+#pragma unroll
+        for (int x = 0; x < kStrips; ++x) {
+            // (not 0: a masked score is -inf)
+            fac[x] = fmaxf(st[x].ks * qf, 1e-37f);
+            float y = s[x / 2][8 * (x & 1)];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) y = fmaxf(y, s[x / 2][8 * (x & 1) + i]);
+            most = fmaxf(most, __builtin_fmaf(y, fac[x], st[x].lv));
+        }
+        if (__any(most > m + 14.0f)) {
+            most = fmaxf(most, xor_lanes(most, 32));
+            const float to = fmaxf(m, most - 6.0f);
+            const float r = __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= r;
+#pragma unroll
+            for (int c = 0; c < CB; ++c) o[c] *= r;
+        }
+        h8_t pr[kStrips];
+#pragma unroll
+        for (int x = 0; x < kStrips; ++x) {
+            const float off = st[x].lv - m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float e = __builtin_amdgcn_exp2f(
+                    __builtin_fmaf(s[x / 2][8 * (x & 1) + i], fac[x], off));
+                sum += e;
+                pr[x][i] = (_Float16)e;
+            }
+            l += sum * st[x].rvs;
         }
 #pragma unroll
         for (int c = 0; c < CB; ++c)
 #pragma unroll
-            for (int x = 0; x < kStrips; ++x) {
-                const h8_t a =
-                    *(const h8_t*)(tile + Tile<D>::kKeys + (x * CB + c) * 1024 + lane * 16);
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
-                    o[rb][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pr[rb][x], o[rb][c], 0, 0, 0);
-            }
+            for (int x = 0; x < kStrips; ++x)
+                o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                    *(const h8_t*)(tile + Tile<D>::kKeys + (x * CB + c) * 1024 + lane * 16), pr[x],
+                    o[c], 0, 0, 0);
     }
 
+    const uint32_t row = seq.row0 + f / p.G;
+    l += xor_lanes(l, 32);
+    if (f >= all_rows || row >= p.rows) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* out = (uint16_t*)p.out + ((uint64_t)row * p.Hq + h * p.G + f % p.G) * D + 4 * half;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        const uint32_t f = f0 + (wave * RB + rb) * 32 + n, row = seq.row0 + f / p.G;
-        const float sum = l[rb] + xor_lanes(l[rb], 32);
-        if (f >= all_rows || row >= p.rows) continue;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        uint16_t* out = (uint16_t*)p.out + ((uint64_t)row * p.Hq + h * p.G + f % p.G) * D + 4 * half;
+    for (int c = 0; c < CB; ++c)
 #pragma unroll
-        for (int c = 0; c < CB; ++c)
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-                *(u2_t*)(out + 32 * c + 8 * x) =
-                    u2_t{narrow2<BF16>(o[rb][c][4 * x] * inv, o[rb][c][4 * x + 1] * inv),
-                         narrow2<BF16>(o[rb][c][4 * x + 2] * inv, o[rb][c][4 * x + 3] * inv)};
-    }
+        for (int x = 0; x < 4; ++x)
+            *(u2_t*)(out + 32 * c + 8 * x) =
+                u2_t{narrow2<BF16>(o[c][4 * x] * inv, o[c][4 * x + 1] * inv),
+                     narrow2<BF16>(o[c][4 * x + 2] * inv, o[c][4 * x + 3] * inv)};
 }
 
-template <int D, int BF16, int INT8, int RB>
+template <int D, int BF16, int INT8, int W>
 hipError_t launch_t(hipStream_t stream, const Kv8AttnParams& p)
 {
     // at most so many tiles: whole ones of all rows, and one more a sequence
     const uint64_t rows = (uint64_t)p.rows * p.G;
-    const uint64_t tiles = rows / group_rows(RB) + (p.B < rows ? p.B : rows);
-    hipLaunchKernelGGL((kv8_prefill<D, BF16, INT8, RB>), dim3((uint32_t)(tiles * p.Hkv)),
-                       dim3(kThreads), 0, stream, p, div_magic(p.S / 16));
+    const uint64_t tiles = rows / group_rows(W) + (p.B < rows ? p.B : rows);
+    hipLaunchKernelGGL((kv8_prefill<D, BF16, INT8, W>), dim3((uint32_t)(tiles * p.Hkv)),
+                       dim3(64 * W), 0, stream, p, div_magic(p.S / 16));
     return hipGetLastError();
 }
 
 template <int D, int BF16, int INT8>
-hipError_t launch_rb(hipStream_t stream, const Kv8AttnParams& p)
+hipError_t launch_w(hipStream_t stream, const Kv8AttnParams& p)
 {
-    // 64 rows of 256 channels and their sums pass a wave's registers
+    // eight waves share a tile's widening; 256 channels fill a wave's registers and
+    // a CU's LDS with four
     if constexpr (D < 256) {
-        if (p.max_q * p.G > 128) return launch_t<D, BF16, INT8, 2>(stream, p);
+        if (p.max_q * p.G > 128) return launch_t<D, BF16, INT8, 8>(stream, p);
     }
-    return launch_t<D, BF16, INT8, 1>(stream, p);
+    return launch_t<D, BF16, INT8, 4>(stream, p);
 }
 
 template <int D>
 hipError_t launch_d(hipStream_t stream, int bf16, int int8, const Kv8AttnParams& p)
 {
-    if (bf16) return int8 ? launch_rb<D, 1, 1>(stream, p) : launch_rb<D, 1, 0>(stream, p);
-    return int8 ? launch_rb<D, 0, 1>(stream, p) : launch_rb<D, 0, 0>(stream, p);
+    if (bf16) return int8 ? launch_w<D, 1, 1>(stream, p) : launch_w<D, 1, 0>(stream, p);
+    return int8 ? launch_w<D, 0, 1>(stream, p) : launch_w<D, 0, 0>(stream, p);
 }
 
 }  // namespace
