@@ -92,6 +92,21 @@ size_t record_bytes(const Cut& c, uint64_t items, uint32_t rec_rows, uint32_t d)
 // the context, split over it, against tiles of 128 and more in LDS.
 bool few_rows(uint64_t rows) { return rows <= 64; }
 
+// The parts that a prefill's row tiles cut their tokens into: with fewer row tiles
+// than the CUs hold at once (two workgroups of four waves, one of eight), as many
+// as fill them, of 512 tokens at least.
+uint32_t prefill_parts(uint32_t d, uint64_t num_rows, uint64_t seqs, uint64_t heads,
+                       uint64_t group, uint64_t max_q, uint64_t cap)
+{
+    const uint64_t waves = tq4::kv8_prefill_waves(d, max_q * group), rows = 32 * waves;
+    uint64_t tiles = mul(seqs, (max_q * group + rows - 1) / rows);
+    if (tiles > mul(num_rows, group) / rows + seqs) tiles = mul(num_rows, group) / rows + seqs;
+    const uint64_t groups = mul(tiles, heads), fit = d < 256 && waves == 4 ? 512 : 256;
+    uint64_t k = groups ? fit / groups : 1;
+    if (k > cap / 512) k = cap / 512;
+    return (uint32_t)(k < 1 ? 1 : k > 64 ? 64 : k);
+}
+
 // The grid and the line of a streamed call's units in bounds.
 bool cut_fits(const Cut& c, uint64_t seqs, uint64_t cap, uint64_t heads, uint64_t tiles)
 {
@@ -299,7 +314,11 @@ size_t tq4_kv8_prefill_workspace_bytes(uint32_t num_rows, uint32_t num_seqs, uin
     if (num_kv_heads == 0) return 0;
     if (max_query_len > num_rows) max_query_len = num_rows;
     const uint64_t group = num_heads / num_kv_heads;
-    if (!few_rows(max_query_len * group)) return 0;
+    if (!few_rows(max_query_len * group)) {
+        const uint32_t k = prefill_parts(head_size, num_rows, num_seqs, num_kv_heads, group,
+                                         max_query_len, (uint64_t)max_blocks_per_seq * block_size);
+        return k == 1 ? 0 : record_bytes(Cut{k, 0, 0}, mul(num_rows, num_heads), 1, head_size);
+    }
     const Cut c = cut_rule(head_size, num_seqs, num_kv_heads, tiles_of(max_query_len, group),
                            (uint64_t)max_blocks_per_seq * block_size, 0);
     return record_bytes(c, mul(num_seqs, num_kv_heads, tiles_of(max_query_len, group)),
@@ -333,19 +352,26 @@ int tq4_kv8_paged_prefill(void* stream, int element_type, int code_type, const v
                     block_size, num_blocks, max_blocks_per_seq, max_query_len, causal != 0, scale,
                     c, workspace);
     };
+    const size_t need =
+        tq4_kv8_prefill_workspace_bytes(num_rows, num_seqs, num_heads, num_kv_heads, head_size,
+                                        block_size, max_blocks_per_seq, max_query_len);
+    const bool room = !need || (workspace && aligned(workspace) && workspace_bytes >= need);
     if (!few_rows(max_query_len * group)) {
-        if (mul(rows / 128 + num_seqs, num_kv_heads) > kMaxGroups) return TQ4_ERR_RANGE;
+        const uint32_t k = prefill_parts(head_size, num_rows, num_seqs, num_kv_heads, group,
+                                         max_query_len, cap);
+        if (mul(mul(rows / 128 + num_seqs, num_kv_heads), k) > kMaxGroups / 2 ||
+            mul(num_rows, num_heads) > kMaxGroups)
+            return TQ4_ERR_RANGE;
+        if (!room) return TQ4_ERR_WORKSPACE;
+        tq4::Kv8AttnParams p = args(Cut{k, 0, 0});
+        p.ml = p.acc + (uint64_t)num_rows * num_heads * k * head_size;
         return launched(tq4::launch_kv8_prefill((hipStream_t)stream, element_type,
-                                                code_type == TQ4_KV8_INT8, args(Cut{1, 0, 0})));
+                                                code_type == TQ4_KV8_INT8, p));
     }
     const Cut s = cut_rule(head_size, num_seqs, num_kv_heads, tiles, cap, 0);
     if (!cut_fits(s, num_seqs, cap, num_kv_heads, tiles) || mul(num_rows, num_heads) > kMaxGroups)
         return TQ4_ERR_RANGE;
-    const size_t need =
-        tq4_kv8_prefill_workspace_bytes(num_rows, num_seqs, num_heads, num_kv_heads, head_size,
-                                        block_size, max_blocks_per_seq, max_query_len);
-    if (need && (!workspace || !aligned(workspace) || workspace_bytes < need))
-        return TQ4_ERR_WORKSPACE;
+    if (!room) return TQ4_ERR_WORKSPACE;
     return launched(tq4::launch_kv8_decode((hipStream_t)stream, element_type,
                                            code_type == TQ4_KV8_INT8, args(s)));
 }

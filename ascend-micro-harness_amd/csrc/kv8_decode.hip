@@ -489,29 +489,19 @@ __global__ __launch_bounds__(kThreads, kKv8GroupsPerCu(D)) void kv8_decode(Kv8At
     }
 }
 
-// The records of a row, weights 2^(m_k - max m): a wave a row, or TEAM of them,
-// which take the records in turn and merge.
+// A row's records, joined by a wave, or by TEAM of them.
 template <int D, int BF16, int TEAM>
-__global__ __launch_bounds__(TEAM > kWaves ? 64 * TEAM : kThreads) void kv8_combine(Kv8AttnParams p, uint32_t max_tiles)
+__global__ __launch_bounds__(TEAM > kWaves ? 64 * TEAM : kThreads) void kv8_combine(
+    Kv8AttnParams p, uint32_t max_tiles)
 {
-    constexpr int C = D / 64;
     __shared__ float part[TEAM > 1 ? TEAM : 1][D];
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
-    const uint32_t mine = wave % TEAM;
-    const uint64_t at = (uint64_t)blockIdx.x * (TEAM < kWaves ? kWaves / TEAM : 1) + wave / TEAM;  // row * Hq + head
+    // row * Hq + head
+    const uint64_t at = (uint64_t)blockIdx.x * (TEAM < kWaves ? kWaves / TEAM : 1) + wave / TEAM;
     const uint32_t row = (uint32_t)(at / p.Hq), hq = (uint32_t)(at % p.Hq);
     if (row >= p.rows) return;
-    uint32_t b = row;
-    if (p.cu) {
-        uint32_t lo = 0, hi = p.B;  // the first sequence that ends past the row
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi) >> 1;
-            if (p.cu[mid + 1] > (int32_t)row) hi = mid;
-            else lo = mid + 1;
-        }
-        b = lo;
-        if (b >= p.B) return;
-    }
+    const uint32_t b = sequence_of(p, row);
+    if (b >= p.B) return;
     const Sequence s(p, b);
     if (row < s.row0 || row - s.row0 >= s.rows) return;
     const uint32_t f = (row - s.row0) * p.G + hq % p.G, h = hq / p.G;
@@ -542,63 +532,9 @@ __global__ __launch_bounds__(TEAM > kWaves ? 64 * TEAM : kThreads) void kv8_comb
         apart = 2;
     }
     if (K < 2) return;  // the whole item went to the output
-    auto record = [&](uint32_t k) {
+    join_records<D, BF16, TEAM>(p, at, K, part, [&](uint32_t k) {
         return (k ? slot + (uint64_t)(k - 1) * apart : slot0) * p.rec_rows + r;
-    };
-    float m = kNone;
-    for (uint32_t k = lane; k < K; k += 64) m = fmaxf(m, p.ml[2 * record(k)]);
-#pragma unroll
-    for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, xor_lanes(m, i));
-    float a[C] = {}, l = 0.0f;
-    for (uint32_t k0 = 0; k0 < K; k0 += 64) {
-        float w = 0.0f;  // of record k0 + lane
-        if (k0 + lane < K) {
-            const float2 x = *(const float2*)(p.ml + 2 * record(k0 + lane));
-            w = __builtin_amdgcn_exp2f(x.x - m);
-            l += w * x.y;
-        }
-        // eight records' loads at a time (past the last: its sums again, weight 0)
-        const uint32_t n = K - k0 < 64 ? K - k0 : 64u;
-        for (uint32_t k = mine; k < n; k += 8 * TEAM) {
-            float x[8][C];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t kj = k + j * TEAM < n ? k + j * TEAM : n - 1;
-                __builtin_memcpy(
-                    x[j], __builtin_assume_aligned(p.acc + record(k0 + kj) * D + lane * C, 4 * C),
-                    4 * C);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const bool in = k + j * TEAM < n;
-                const float wk = __uint_as_float(__builtin_amdgcn_readlane(
-                    __float_as_uint(w), in ? k + j * TEAM : 0));
-#pragma unroll
-                for (int i = 0; i < C; ++i) a[i] = in ? a[i] + wk * x[j][i] : a[i];
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 1; i < 64; i <<= 1) l += xor_lanes(l, i);
-    if constexpr (TEAM > 1) {
-#pragma unroll
-        for (int i = 0; i < C; ++i) part[mine][lane * C + i] = a[i];
-        __syncthreads();
-        if (mine) return;
-#pragma unroll
-        for (int t = 1; t < TEAM; ++t)
-#pragma unroll
-            for (int i = 0; i < C; ++i) a[i] += part[t][lane * C + i];
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* out = (uint16_t*)p.out + at * D + lane * C;
-    if constexpr (C == 1) {
-        *out = (uint16_t)narrow2<BF16>(a[0] * inv, 0.0f);
-    } else {
-#pragma unroll
-        for (int i = 0; i < C; i += 2)
-            *(uint32_t*)(out + i) = narrow2<BF16>(a[i] * inv, a[i + 1] * inv);
-    }
+    });
 }
 
 template <int D, int BF16, int INT8>

@@ -156,5 +156,83 @@ struct SequenceBase {
     }
 };
 
+// The sequence that a row belongs to: the first that ends past it.
+__device__ __forceinline__ uint32_t sequence_of(const Kv8AttnParams& p, uint32_t row)
+{
+    if (!p.cu) return row;
+    uint32_t lo = 0, hi = p.B;
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (p.cu[mid + 1] > (int32_t)row) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+// The K records of output row `at`, weights 2^(m_k - max m), to the output. TEAM
+// waves take them in turn and merge in `part` (TEAM rows; one wave: not used);
+// record(k): the index of record k.
+template <int D, int BF16, int TEAM, class Record>
+__device__ __forceinline__ void join_records(const Kv8AttnParams& p, uint64_t at, uint32_t K,
+                                             float (*part)[D], Record&& record)
+{
+    constexpr int C = D / 64;
+    const uint32_t lane = threadIdx.x & 63u, mine = (threadIdx.x >> 6) % TEAM;
+    float m = kNone;
+    for (uint32_t k = lane; k < K; k += 64) m = fmaxf(m, p.ml[2 * record(k)]);
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, xor_lanes(m, i));
+    float a[C] = {}, l = 0.0f;
+    for (uint32_t k0 = 0; k0 < K; k0 += 64) {
+        float w = 0.0f;  // of record k0 + lane
+        if (k0 + lane < K) {
+            const float2 x = *(const float2*)(p.ml + 2 * record(k0 + lane));
+            w = __builtin_amdgcn_exp2f(x.x - m);
+            l += w * x.y;
+        }
+        // eight records' loads at a time (past the last: its sums again, weight 0)
+        const uint32_t n = K - k0 < 64 ? K - k0 : 64u;
+        for (uint32_t k = mine; k < n; k += 8 * TEAM) {
+            float x[8][C];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t kj = k + j * TEAM < n ? k + j * TEAM : n - 1;
+                __builtin_memcpy(
+                    x[j], __builtin_assume_aligned(p.acc + record(k0 + kj) * D + lane * C, 4 * C),
+                    4 * C);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool in = k + j * TEAM < n;
+                const float wk = __uint_as_float(
+                    __builtin_amdgcn_readlane(__float_as_uint(w), in ? k + j * TEAM : 0));
+#pragma unroll
+                for (int i = 0; i < C; ++i) a[i] = in ? a[i] + wk * x[j][i] : a[i];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) l += xor_lanes(l, i);
+    if constexpr (TEAM > 1) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) part[mine][lane * C + i] = a[i];
+        __syncthreads();
+        if (mine) return;
+#pragma unroll
+        for (int t = 1; t < TEAM; ++t)
+#pragma unroll
+            for (int i = 0; i < C; ++i) a[i] += part[t][lane * C + i];
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* out = (uint16_t*)p.out + at * D + lane * C;
+    if constexpr (C == 1) {
+        *out = (uint16_t)narrow2<BF16>(a[0] * inv, 0.0f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; i += 2)
+            *(uint32_t*)(out + i) = narrow2<BF16>(a[i] * inv, a[i + 1] * inv);
+    }
+}
+
 }  // namespace kv8
 }  // namespace tq4

@@ -52,6 +52,10 @@ struct Kv8AttnParams {
     int causal;
     float scale;
 };
+// Waves of a prefill workgroup, 32 rows each (kv8_prefill.hip), for so many rows of
+// a (sequence, kv head).
+inline uint32_t kv8_prefill_waves(uint32_t d, uint64_t rows) { return d < 256 && rows > 128 ? 8 : 4; }
+
 hipError_t launch_kv8_decode(hipStream_t stream, int bf16, int int8, const Kv8AttnParams& p);
 hipError_t launch_kv8_prefill(hipStream_t stream, int bf16, int int8, const Kv8AttnParams& p);
 

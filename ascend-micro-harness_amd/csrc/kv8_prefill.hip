@@ -141,6 +141,25 @@ struct Stage {
     }
 };
 
+// The token tiles that some row of a row tile sees, and those of each of its K
+// parts.
+struct Span {
+    uint32_t tiles, each;
+
+    __device__ __forceinline__ Span(const Kv8AttnParams& p, const SequenceBase& seq, uint32_t f0,
+                                    uint32_t rows)
+    {
+        uint32_t end = seq.tokens;
+        if (p.causal) {
+            const uint32_t all = seq.rows * p.G, last = f0 + rows < all ? f0 + rows - 1 : all - 1;
+            const int64_t x = (int64_t)seq.tokens - seq.all + last / p.G + 1;
+            end = x < 0 ? 0u : (uint32_t)x;
+        }
+        tiles = (end + kTile - 1) / kTile;
+        each = (tiles + p.K - 1) / p.K;
+    }
+};
+
 template <int D, int BF16, int INT8, int W>
 __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnParams p,
                                                                        Divisor per_page)
@@ -152,9 +171,10 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
     const uint32_t n = lane & 31u, half = lane >> 5;
 
     // the heads of a tile lie next to each other in the grid (one an XCD, where
-    // there are eight); a sequence's last tiles, the longest, come first
-    const uint32_t h = blockIdx.x % p.Hkv;
-    uint32_t t = gridDim.x / p.Hkv - 1 - blockIdx.x / p.Hkv, b = 0;
+    // there are eight), then the parts of its tokens; a sequence's last tiles, the
+    // longest, come first
+    const uint32_t h = blockIdx.x % p.Hkv, part = blockIdx.x / p.Hkv % p.K;
+    uint32_t t = gridDim.x / (p.Hkv * p.K) - 1 - blockIdx.x / (p.Hkv * p.K), b = 0;
     SequenceBase seq;
     {
         uint32_t before = 0;
@@ -221,13 +241,9 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
             for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
     }
 
-    // tokens that the workgroup's rows see, and that every row of the wave sees
-    const uint32_t last = f0 + group_rows(W) < all_rows ? f0 + group_rows(W) - 1 : all_rows - 1;
-    uint32_t end = seq.tokens;
+    // tokens that every row of the wave sees, and that some row does
     int32_t whole = (int32_t)seq.tokens, some = (int32_t)seq.tokens;
     if (p.causal) {
-        const int64_t x = (int64_t)seq.tokens - seq.all + last / p.G + 1;
-        end = x < 0 ? 0u : (uint32_t)x;
         const uint32_t wf = f0 + wave * 32;
         const int64_t y = (int64_t)seq.tokens - seq.all + wf / p.G + 1;
         whole = y < 0 ? 0 : y < seq.tokens ? (int32_t)y : (int32_t)seq.tokens;
@@ -235,27 +251,30 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
         some = z < 0 ? 0 : z < seq.tokens ? (int32_t)z : (int32_t)seq.tokens;
     }
     if (f0 + wave * 32 >= all_rows) some = 0;  // no row of its own
-    const uint32_t tiles = (end + kTile - 1) / kTile;
+    const Span span(p, seq, f0, group_rows(W));
+    const uint32_t first = part * span.each;
+    if (part && first >= span.tiles) return;
+    const uint32_t end = first + span.each < span.tiles ? first + span.each : span.tiles;
 
     Stage<D, INT8, W> stage;
-    if (tiles) {
-        stage.entries(p, table, per_page, 0);
-        stage.fetch(p, per_page, h, seq.tokens, 0);
-        stage.store(lds, info[0]);
+    if (first < end) {
+        stage.entries(p, table, per_page, first * kTile);
+        stage.fetch(p, per_page, h, seq.tokens, first * kTile);
+        stage.store(lds + (first & 1) * Tile<D>::kBytes, info[first & 1]);
     }
-    if (tiles > 1) {
-        stage.entries(p, table, per_page, kTile);
-        stage.fetch(p, per_page, h, seq.tokens, kTile);
-        stage.entries(p, table, per_page, 2 * kTile);
+    if (first + 1 < end) {
+        stage.entries(p, table, per_page, (first + 1) * kTile);
+        stage.fetch(p, per_page, h, seq.tokens, (first + 1) * kTile);
+        stage.entries(p, table, per_page, (first + 2) * kTile);
     }
-    for (uint32_t j = 0; j < tiles; ++j) {
+    for (uint32_t j = first; j < end; ++j) {
         __syncthreads();  // tile j is in LDS, the other buffer has been read
         char* tile = lds + (j & 1) * Tile<D>::kBytes;
         const StripInfo* at = info[j & 1];
         const int32_t t0 = (int32_t)(j * kTile);
-        if (j + 1 < tiles) {
+        if (j + 1 < end) {
             stage.store(lds + ((j + 1) & 1) * Tile<D>::kBytes, info[(j + 1) & 1]);
-            if (j + 2 < tiles) {
+            if (j + 2 < end) {
                 // (the entries of tile j + 2 came a tile ago)
                 stage.fetch(p, per_page, h, seq.tokens, t0 + 2 * kTile);
                 stage.entries(p, table, per_page, t0 + 3 * kTile);
@@ -339,8 +358,23 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
     const uint32_t row = seq.row0 + f / p.G;
     l += xor_lanes(l, 32);
     if (f >= all_rows || row >= p.rows) return;
+    const uint64_t to = (uint64_t)row * p.Hq + h * p.G + f % p.G;
+    if (span.each < span.tiles) {
+        const uint64_t rec = to * p.K + part;
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                *(f4_t*)(p.acc + rec * D + 32 * c + 8 * x + 4 * half) =
+                    f4_t{o[c][4 * x], o[c][4 * x + 1], o[c][4 * x + 2], o[c][4 * x + 3]};
+        if (half == 0) {
+            p.ml[2 * rec] = m;
+            p.ml[2 * rec + 1] = l;
+        }
+        return;
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* out = (uint16_t*)p.out + ((uint64_t)row * p.Hq + h * p.G + f % p.G) * D + 4 * half;
+    uint16_t* out = (uint16_t*)p.out + to * D + 4 * half;
 #pragma unroll
     for (int c = 0; c < CB; ++c)
 #pragma unroll
@@ -350,14 +384,36 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
                      narrow2<BF16>(o[c][4 * x + 2] * inv, o[c][4 * x + 3] * inv)};
 }
 
+// The parts of a row, a wave each row.
+template <int D, int BF16, int W>
+__global__ __launch_bounds__(256) void kv8_prefill_combine(Kv8AttnParams p)
+{
+    const uint64_t at = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // row * Hq + head
+    const uint32_t row = (uint32_t)(at / p.Hq), hq = (uint32_t)(at % p.Hq);
+    if (row >= p.rows) return;
+    const uint32_t b = sequence_of(p, row);
+    if (b >= p.B) return;
+    const SequenceBase s(p, b);
+    if (row < s.row0 || row - s.row0 >= s.rows) return;
+    const uint32_t f = (row - s.row0) * p.G + hq % p.G;
+    const Span span(p, s, f / group_rows(W) * group_rows(W), group_rows(W));
+    if (span.each >= span.tiles) return;  // one part: it went to the output
+    const uint32_t parts = (span.tiles + span.each - 1) / span.each;
+    join_records<D, BF16, 1>(p, at, parts, nullptr, [&](uint32_t k) { return at * p.K + k; });
+}
+
 template <int D, int BF16, int INT8, int W>
 hipError_t launch_t(hipStream_t stream, const Kv8AttnParams& p)
 {
     // at most so many tiles: whole ones of all rows, and one more a sequence
     const uint64_t rows = (uint64_t)p.rows * p.G;
     const uint64_t tiles = rows / group_rows(W) + (p.B < rows ? p.B : rows);
-    hipLaunchKernelGGL((kv8_prefill<D, BF16, INT8, W>), dim3((uint32_t)(tiles * p.Hkv)),
+    hipLaunchKernelGGL((kv8_prefill<D, BF16, INT8, W>), dim3((uint32_t)(tiles * p.K * p.Hkv)),
                        dim3(64 * W), 0, stream, p, div_magic(p.S / 16));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.K == 1) return e;
+    hipLaunchKernelGGL((kv8_prefill_combine<D, BF16, W>),
+                       dim3((uint32_t)(((uint64_t)p.rows * p.Hq + 3) / 4)), dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 
@@ -367,7 +423,8 @@ hipError_t launch_w(hipStream_t stream, const Kv8AttnParams& p)
     // eight waves share a tile's widening; 256 channels fill a wave's registers and
     // a CU's LDS with four
     if constexpr (D < 256) {
-        if (p.max_q * p.G > 128) return launch_t<D, BF16, INT8, 8>(stream, p);
+        if (kv8_prefill_waves(D, (uint64_t)p.max_q * p.G) == 8)
+            return launch_t<D, BF16, INT8, 8>(stream, p);
     }
     return launch_t<D, BF16, INT8, 4>(stream, p);
 }

@@ -267,6 +267,20 @@ def test_prefill_few_rows_of_long_contexts(tq4, causal):
         check_prefill(tq4, queries(r, sum(rows), 2 * G, d, "bf16"), c, lens, rows, "fp8", causal)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d,G,rows,lens", [(128, 4, [70, 20], [2600, 1]), (64, 2, [100], [4100]),
+                                           (256, 8, [40, 9, 0], [1500, 700, 300]),
+                                           (128, 1, [300, 129, 1], [1800, 2000, 1100])])
+def test_prefill_parts(tq4, d, G, rows, lens, causal):
+    """Row tiles too few for the GPU: their contexts are cut into parts and joined."""
+    r = np.random.default_rng(d + G)
+    lens = [max(a, b) for a, b in zip(lens, rows)]
+    c = cache(r, lens, 1, 32, d, "int8")
+    assert tq4.kv8_prefill_workspace_bytes(sum(rows), len(rows), G, 1, d, 32, c[3].shape[1],
+                                           max(rows)) > 0
+    check_prefill(tq4, queries(r, sum(rows) + 1, G, d, "fp16"), c, lens, rows, "int8", causal)
+
+
 def test_prefill_wrong_lengths_stay_inside(tq4):
     """max_query_len below a sequence's rows: the rows past it are left; pages
     that name nothing in the middle; contexts past the table."""
