@@ -51,21 +51,32 @@ struct StripInfo {
 
 // What a thread brings of a tile: N pieces of 16 bytes of each plane, of 4 * D. Key
 // piece u: token u / (D / 16), channels 16 * (u % (D / 16)) ..; value piece u:
-// strip u / D, channel u % D.
+// strip u / D, channel u % D. Both planes' pieces u lie in strip u / D of the tile,
+// which is one strip for a wave: pages and addresses are scalars.
 template <int D, int INT8, int W>
 struct Stage {
     static constexpr int kThreads = 64 * W, kPieces = 4 * D;
     static constexpr int N = (kPieces + kThreads - 1) / kThreads;
     u4_t k[N], v[N];
-    int live[N];      // live tokens of the value pieces' strips
-    int32_t e[N], es;  // the next fetch's block-table entries, -1: no page
-    float ks, vs;      // of strip threadIdx.x, its live tokens
+    int live[N];    // live tokens of the pieces' strips
+    int32_t e[N];   // the next fetch's block-table entries, -1: no page
+    int32_t es;     // the same of strip threadIdx.x % 4, its scales and live tokens
+    float ks, vs;
     int own;
 
-    // (a thread too many brings another's piece, and does not store it)
+    // (a wave too many brings another's pieces, and does not store them)
     static __device__ __forceinline__ uint32_t piece(int r)
     {
         return (r * kThreads + threadIdx.x) % kPieces;
+    }
+    static __device__ __forceinline__ uint32_t strip_of(int r)
+    {
+        return __builtin_amdgcn_readfirstlane(piece(r) / D);
+    }
+    static __device__ __forceinline__ int live_of(int32_t e, uint32_t L, uint32_t strip)
+    {
+        const int left = (int)L - (int)(16 * strip);
+        return e < 0 || left < 0 ? 0 : left > 16 ? 16 : left;
     }
 
     __device__ __forceinline__ int32_t entry(const Kv8AttnParams& p, const int32_t* table,
@@ -79,10 +90,7 @@ struct Stage {
                                             Divisor per_page, uint32_t t0)
     {
 #pragma unroll
-        for (int r = 0; r < N; ++r) {
-            // both planes' pieces u lie in strip u / D of the tile
-            e[r] = entry(p, table, per_page, t0 / 16 + piece(r) / D);
-        }
+        for (int r = 0; r < N; ++r) e[r] = entry(p, table, per_page, t0 / 16 + strip_of(r));
         es = entry(p, table, per_page, t0 / 16 + (threadIdx.x & 3u));
     }
     __device__ __forceinline__ void fetch(const Kv8AttnParams& p, Divisor per_page, uint32_t h,
@@ -90,22 +98,20 @@ struct Stage {
     {
 #pragma unroll
         for (int r = 0; r < N; ++r) {
-            const uint32_t u = piece(r);
-            const uint32_t strip = t0 / 16 + u / D;
+            const uint32_t u = piece(r), strip = t0 / 16 + strip_of(r);
+            const int32_t page = __builtin_amdgcn_readfirstlane(e[r]);
             const uint32_t in = strip - div_by(strip, per_page) * (p.S / 16);
-            const uint64_t row = (uint64_t)(uint32_t)(e[r] < 0 ? 0 : e[r]) * p.Hkv + h;
-            const uint32_t token = u / (D / 16) % 16;
-            k[r] = *(const u4_t*)(p.key_cache + (row * p.S + in * 16 + token) * D +
-                                  16 * (u % (D / 16)));
-            v[r] = *(const u4_t*)(p.value_cache + (row * p.S + in * 16) * D + 16 * (u % D));
-            const int left = (int)L - (int)(16 * strip);
-            live[r] = e[r] < 0 || left < 0 ? 0 : left > 16 ? 16 : left;
+            const uint64_t at =
+                (((uint64_t)(uint32_t)(page < 0 ? 0 : page) * p.Hkv + h) * p.S + in * 16) * D;
+            // a strip's keys and values are 16 * D consecutive bytes, its pieces in order
+            k[r] = *(const u4_t*)(p.key_cache + at + 16 * (u % D));
+            v[r] = *(const u4_t*)(p.value_cache + at + 16 * (u % D));
+            live[r] = live_of(page, L, strip);
         }
         const uint64_t row = (uint64_t)(uint32_t)(es < 0 ? 0 : es) * p.Hkv + h;
         ks = p.scales[row];
         vs = p.scales[(uint64_t)p.P * p.Hkv + row];
-        const int left = (int)L - (int)(t0 + 16 * (threadIdx.x & 3u));
-        own = es < 0 || left < 0 ? 0 : left > 16 ? 16 : left;
+        own = live_of(es, L, t0 / 16 + (threadIdx.x & 3u));
     }
     __device__ __forceinline__ void store(char* tile, StripInfo* info) const
     {
@@ -122,7 +128,8 @@ struct Stage {
             }
             {
                 // a dead token's bytes may be a NaN: 0 times it is not 0
-                const u4_t w = live[r] < 16 ? live_bytes(v[r], live[r]) : v[r];
+                u4_t w = v[r];
+                if (live[r] < 16) w = live_bytes(w, live[r]);
                 const uint32_t strip = u / D, c = u % D;
                 char* to = tile + Tile<D>::kKeys + (strip * (D / 32) + c / 32) * 1024 + (c % 32) * 16;
                 *(h8_t*)to = widen8<INT8>(w[0], w[1]);
