@@ -93,17 +93,16 @@ size_t record_bytes(const Cut& c, uint64_t items, uint32_t rec_rows, uint32_t d)
 bool few_rows(uint64_t rows) { return rows <= 64; }
 
 // The parts that a prefill's row tiles cut their tokens into: with fewer row tiles
-// than the CUs hold at once (two workgroups of four waves, one of eight), as many
-// as fill them, of 512 tokens at least.
+// than the CUs hold at once, as many as fill them, of 256 tokens at least.
 uint32_t prefill_parts(uint32_t d, uint64_t num_rows, uint64_t seqs, uint64_t heads,
                        uint64_t group, uint64_t max_q, uint64_t cap)
 {
     const uint64_t waves = tq4::kv8_prefill_waves(d, max_q * group), rows = 32 * waves;
     uint64_t tiles = mul(seqs, (max_q * group + rows - 1) / rows);
     if (tiles > mul(num_rows, group) / rows + seqs) tiles = mul(num_rows, group) / rows + seqs;
-    const uint64_t groups = mul(tiles, heads), fit = d < 256 && waves == 4 ? 512 : 256;
-    uint64_t k = groups ? fit / groups : 1;
-    if (k > cap / 512) k = cap / 512;
+    const uint64_t groups = mul(tiles, heads);
+    uint64_t k = groups ? tq4::kv8_prefill_fit(d, (uint32_t)waves) / groups : 1;
+    if (k > cap / 256) k = cap / 256;
     return (uint32_t)(k < 1 ? 1 : k > 64 ? 64 : k);
 }
 

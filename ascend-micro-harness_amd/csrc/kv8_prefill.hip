@@ -1,7 +1,7 @@
 // kv8_prefill.hip -- attention of many rows a sequence over the 8-bit paged cache
 // (tq4_kv8_paged_prefill of prompt chunks and cross attention; tq4_kv8.h).
 //
-// A workgroup takes 256 (or 128) rows of a (sequence, kv head): query tokens times
+// A workgroup takes 128 (or 256) rows of a (sequence, kv head): query tokens times
 // the GQA group's heads, so the group shares each key. A wave has 32 of them and
 // walks the tokens 64 at a time with its workgroup:
 //   S = K Q^T       MFMA 32x32x16 f16, 32 tokens x 32 rows
@@ -427,9 +427,7 @@ hipError_t launch_t(hipStream_t stream, const Kv8AttnParams& p)
 template <int D, int BF16, int INT8>
 hipError_t launch_w(hipStream_t stream, const Kv8AttnParams& p)
 {
-    // eight waves share a tile's widening; 256 channels fill a wave's registers and
-    // a CU's LDS with four
-    if constexpr (D < 256) {
+    if constexpr (D == 128) {
         if (kv8_prefill_waves(D, (uint64_t)p.max_q * p.G) == 8)
             return launch_t<D, BF16, INT8, 8>(stream, p);
     }
