@@ -90,7 +90,9 @@ struct Stage {
                                             Divisor per_page, uint32_t t0)
     {
 #pragma unroll
-        for (int r = 0; r < N; ++r) e[r] = entry(p, table, per_page, t0 / 16 + strip_of(r));
+        // (a vector load, though one entry a wave: a scalar one is waited for together
+        // with the wave's LDS reads)
+        for (int r = 0; r < N; ++r) e[r] = entry(p, table, per_page, t0 / 16 + piece(r) / D);
         es = entry(p, table, per_page, t0 / 16 + (threadIdx.x & 3u));
     }
     __device__ __forceinline__ void fetch(const Kv8AttnParams& p, Divisor per_page, uint32_t h,
@@ -391,22 +393,60 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
                      narrow2<BF16>(o[c][4 * x + 2] * inv, o[c][4 * x + 3] * inv)};
 }
 
-// The parts of a row, a wave each row.
+// The parts of the rows, joined: D / 4 lanes a (row, head), as many workgroups as a
+// launch carries without their number counting (32000 rows x heads on a wave each
+// took 32 us, 4 ns a workgroup).
+constexpr uint32_t kJoinGroups = 1024;
+
 template <int D, int BF16, int W>
 __global__ __launch_bounds__(256) void kv8_prefill_combine(Kv8AttnParams p)
 {
-    const uint64_t at = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // row * Hq + head
-    const uint32_t row = (uint32_t)(at / p.Hq), hq = (uint32_t)(at % p.Hq);
-    if (row >= p.rows) return;
-    const uint32_t b = sequence_of(p, row);
-    if (b >= p.B) return;
-    const SequenceBase s(p, b);
-    if (row < s.row0 || row - s.row0 >= s.rows) return;
-    const uint32_t f = (row - s.row0) * p.G + hq % p.G;
-    const Span span(p, s, f / group_rows(W) * group_rows(W), group_rows(W));
-    if (span.each >= span.tiles) return;  // one part: it went to the output
-    const uint32_t parts = (span.tiles + span.each - 1) / span.each;
-    join_records<D, BF16, 1>(p, at, parts, nullptr, [&](uint32_t k) { return at * p.K + k; });
+    constexpr uint32_t kLanes = D / 4, kPer = 256 / kLanes;
+    const uint64_t all = (uint64_t)p.rows * p.Hq;
+    const uint32_t ch = threadIdx.x % kLanes * 4;
+    for (uint64_t at = (uint64_t)blockIdx.x * kPer + threadIdx.x / kLanes; at < all;
+         at += (uint64_t)gridDim.x * kPer) {  // row * Hq + head
+        const uint32_t row = (uint32_t)(at / p.Hq), hq = (uint32_t)(at % p.Hq);
+        const uint32_t b = sequence_of(p, row);
+        if (b >= p.B) continue;
+        const SequenceBase s(p, b);
+        if (row < s.row0 || row - s.row0 >= s.rows) continue;
+        const uint32_t f = (row - s.row0) * p.G + hq % p.G;
+        const Span span(p, s, f / group_rows(W) * group_rows(W), group_rows(W));
+        if (span.each >= span.tiles) continue;  // one part: it went to the output
+        const uint32_t parts = (span.tiles + span.each - 1) / span.each;
+        const float* ml = p.ml + 2 * at * p.K;
+        // eight parts' loads at a time (past the last: its own again, left out)
+        float m = kNone, l = 0.0f;
+        f4_t a = {0, 0, 0, 0};
+        for (uint32_t k0 = 0; k0 < parts; k0 += 8) {
+            float2 st[8];
+            f4_t x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t k = k0 + j < parts ? k0 + j : parts - 1;
+                st[j] = *(const float2*)(ml + 2 * k);
+                x[j] = *(const f4_t*)(p.acc + (at * p.K + k) * D + ch);
+            }
+            float to = m;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) to = fmaxf(to, st[j].x);
+            const float r = __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= r;
+            a *= r;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (k0 + j >= parts) break;
+                const float w = __builtin_amdgcn_exp2f(st[j].x - m);
+                l += w * st[j].y;
+                a += w * x[j];
+            }
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        *(u2_t*)((uint16_t*)p.out + at * D + ch) =
+            u2_t{narrow2<BF16>(a[0] * inv, a[1] * inv), narrow2<BF16>(a[2] * inv, a[3] * inv)};
+    }
 }
 
 template <int D, int BF16, int INT8, int W>
@@ -419,8 +459,10 @@ hipError_t launch_t(hipStream_t stream, const Kv8AttnParams& p)
                        dim3(64 * W), 0, stream, p, div_magic(p.S / 16));
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.K == 1) return e;
+    const uint64_t joins = ((uint64_t)p.rows * p.Hq * (D / 4) + 255) / 256;
     hipLaunchKernelGGL((kv8_prefill_combine<D, BF16, W>),
-                       dim3((uint32_t)(((uint64_t)p.rows * p.Hq + 3) / 4)), dim3(256), 0, stream, p);
+                       dim3(joins < kJoinGroups ? (uint32_t)joins : kJoinGroups), dim3(256), 0,
+                       stream, p);
     return hipGetLastError();
 }
 
