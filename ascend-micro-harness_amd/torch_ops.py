@@ -17,6 +17,10 @@ argument lists follow the reference's vLLM-style entry points
                            (op_adapter/turboquant_torch_adpt.h:12-22,
                            turboquant_torch_ops.h:6-7)
 
+and those of the 8-bit paged cache, which the reference lacks: tq4::paged_plan,
+tq4::kv8_reshape_and_cache, tq4::kv8_paged_decode and tq4::kv8_paged_prefill
+(include/tq4_kv8.h; shapes and types as in `kv8`).
+
 Sizes that the reference passes as integers (num_tokens, num_kv_heads,
 head_size, num_heads, max_blocks_per_seq, num_blocks) come from tensor shapes
 here. Caches are the TQ4 byte pools: key_cache and value_cache int8
@@ -37,6 +41,7 @@ from typing import Optional
 
 import torch
 
+from . import kv8 as _kv8
 from . import tq4 as _tq4
 
 NAMESPACE = "tq4"
@@ -207,6 +212,75 @@ def _(query, pi_signs, gate, query_rot, key_cache, value_cache, scale_cache, blo
     return torch.empty_like(query)
 
 
+@torch.library.custom_op(
+    f"{NAMESPACE}::paged_plan", device_types="cuda",
+    mutates_args=("context_lens", "block_tables", "free_pages", "free_state", "slot_mapping",
+                  "positions", "cu_seqlens", "granted"))
+def paged_plan(context_lens: torch.Tensor, query_lens: torch.Tensor,
+               release: Optional[torch.Tensor], block_tables: torch.Tensor,
+               free_pages: torch.Tensor, free_state: torch.Tensor, slot_mapping: torch.Tensor,
+               positions: torch.Tensor, cu_seqlens: torch.Tensor, granted: torch.Tensor,
+               block_size: int) -> None:
+    """The page plan of a step, lengths and ring state in place (all int32)."""
+    _kv8.paged_plan(context_lens, query_lens, block_tables, free_pages, free_state, slot_mapping,
+                    cu_seqlens, granted, block_size, release=release, positions=positions)
+
+
+@paged_plan.register_fake
+def _(context_lens, query_lens, release, block_tables, free_pages, free_state, slot_mapping,
+      positions, cu_seqlens, granted, block_size):
+    return None
+
+
+@torch.library.custom_op(f"{NAMESPACE}::kv8_reshape_and_cache",
+                         mutates_args=("key_cache", "value_cache", "scale_cache"),
+                         device_types="cuda")
+def kv8_reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
+                          value_cache: torch.Tensor, scale_cache: torch.Tensor,
+                          slot_mapping: torch.Tensor) -> None:
+    """BF16 or FP16 rows into the 8-bit cache at slot_mapping."""
+    _kv8.kv8_reshape_and_cache(key, value, key_cache, value_cache, scale_cache, slot_mapping)
+
+
+@kv8_reshape_and_cache.register_fake
+def _(key, value, key_cache, value_cache, scale_cache, slot_mapping):
+    return None
+
+
+@torch.library.custom_op(f"{NAMESPACE}::kv8_paged_decode", mutates_args=(), device_types="cuda")
+def kv8_paged_decode(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                     scale_cache: torch.Tensor, block_tables: torch.Tensor,
+                     context_lens: torch.Tensor, num_splits: int, scale: float) -> torch.Tensor:
+    """One row a sequence over the 8-bit cache; scale 0 means 1/sqrt(head_size)."""
+    return _kv8.kv8_paged_decode(query, key_cache, value_cache, scale_cache, block_tables,
+                                 context_lens, num_splits=num_splits,
+                                 scale=scale if scale != 0.0 else None)
+
+
+@kv8_paged_decode.register_fake
+def _(query, key_cache, value_cache, scale_cache, block_tables, context_lens, num_splits, scale):
+    return torch.empty(query.shape, dtype=query.dtype, device=query.device)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::kv8_paged_prefill", mutates_args=(), device_types="cuda")
+def kv8_paged_prefill(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                      scale_cache: torch.Tensor, block_tables: torch.Tensor,
+                      context_lens: torch.Tensor, cu_seqlens: torch.Tensor, max_query_len: int,
+                      causal: bool, scale: float) -> torch.Tensor:
+    """Several rows a sequence over the 8-bit cache; rows of no sequence are 0;
+    scale 0 means 1/sqrt(head_size)."""
+    out = torch.zeros(query.shape, dtype=query.dtype, device=query.device)
+    return _kv8.kv8_paged_prefill(query, key_cache, value_cache, scale_cache, block_tables,
+                                  context_lens, cu_seqlens, max_query_len, causal=causal, out=out,
+                                  scale=scale if scale != 0.0 else None)
+
+
+@kv8_paged_prefill.register_fake
+def _(query, key_cache, value_cache, scale_cache, block_tables, context_lens, cu_seqlens,
+      max_query_len, causal, scale):
+    return torch.empty(query.shape, dtype=query.dtype, device=query.device)
+
+
 def kv4fp8_workspace_for(query: torch.Tensor, num_kv_heads: int, block_tables: torch.Tensor,
                          block_size: int, num_blocks: int = 1) -> torch.Tensor:
     """A zeroed workspace for tq4::fused_decode_opt(_raw_query) at this
@@ -232,4 +306,5 @@ def workspace_for(query: torch.Tensor, num_kv_heads: int, block_tables: torch.Te
 
 __all__ = ["NAMESPACE", "reshape_and_cache", "reshape_scatter", "paged_attention",
            "workspace_for", "fused_decode_opt", "fused_decode_opt_raw_query",
-           "kv4fp8_workspace_for"]
+           "kv4fp8_workspace_for", "paged_plan", "kv8_reshape_and_cache", "kv8_paged_decode",
+           "kv8_paged_prefill"]

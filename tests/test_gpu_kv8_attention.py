@@ -360,6 +360,27 @@ def test_steps_of_plan_write_attend(tq4, code, dtype):
     assert sum(kept.values()) > 200
 
 
+def test_torch_ops(tq4):
+    """The registered operators give the entry points' results."""
+    r = np.random.default_rng(30)
+    ops, lens = torch.ops.tq4, [70, 1]
+    kc, vc, sc = tq4.kv8_cache(12, 1, 16, 64)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=DEV)  # noqa: E731
+    ctx, tables, ring = i32(2), i32(2, 6), dev(r.permutation(12).astype(np.int32))
+    slots, pos, cu, granted = i32(73), i32(73), i32(3), i32(2)
+    ops.paged_plan(ctx, dev(np.array(lens, np.int32)), None, tables, ring,
+                   dev(np.array([0, 12], np.int32)), slots, pos, cu, granted, 16)
+    assert ctx.tolist() == lens == granted.tolist() and cu.tolist() == [0, 70, 71]
+    k, v = queries(r, 73, 1, 64, "fp16").to(DEV), queries(r, 73, 1, 64, "fp16").to(DEV)
+    ops.kv8_reshape_and_cache(k, v, kc, vc, sc, slots)
+    q = queries(r, 73, 2, 64, "fp16").to(DEV)
+    out = ops.kv8_paged_prefill(q, kc, vc, sc, tables, ctx, cu, 70, True, 0.0)
+    want = tq4.kv8_paged_prefill(q, kc, vc, sc, tables, ctx, cu, 70)
+    assert torch.equal(out[:71], want[:71]) and (out[71:] == 0).all()
+    assert torch.equal(ops.kv8_paged_decode(q[:2], kc, vc, sc, tables, ctx, 2, 0.3),
+                       tq4.kv8_paged_decode(q[:2], kc, vc, sc, tables, ctx, num_splits=2, scale=0.3))
+
+
 def test_captured_step(tq4):
     """A captured step (write, decode, split and not), replayed with eager work
     between, gives the eager bits every time; two graphs have their own workspaces."""
@@ -389,6 +410,33 @@ def test_captured_step(tq4):
             out.zero_()
             g.replay()
             eager = tq4.kv8_paged_decode(q, kc, vc, sc, tables, L, num_splits=K)
+            torch.cuda.synchronize()
+            assert torch.equal(out, eager)
+
+
+def test_captured_prefill(tq4):
+    """Captured prefills, in parts and streamed, replayed with eager work between."""
+    r = np.random.default_rng(23)
+    lens, rows = [2100, 1500], [100, 30]
+    c = cache(r, lens, 1, 16, 128, "fp8")
+    kc, vc, sc, tables = on_device(*c, "fp8")
+    L = dev(np.array(lens, np.int32))
+    for n in (rows, [3, 4]):
+        cu = dev(np.concatenate([[0], np.cumsum(n)]).astype(np.int32))
+        q = queries(r, sum(n), 4, 128, "bf16").to(DEV)
+        out = torch.empty_like(q)
+        size = tq4.kv8_prefill_workspace_bytes(sum(n), 2, 4, 1, 128, 16, tables.shape[1], max(n))
+        ws = torch.full((size,), 255, dtype=torch.uint8, device=DEV)
+        assert size > 0
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            tq4.kv8_paged_prefill(q, kc, vc, sc, tables, L, cu, max(n), out=out, workspace=ws)
+        for _ in range(3):
+            q.copy_(queries(r, sum(n), 4, 128, "bf16"))
+            out.zero_()
+            g.replay()
+            eager = tq4.kv8_paged_prefill(q, kc, vc, sc, tables, L, cu, max(n))
             torch.cuda.synchronize()
             assert torch.equal(out, eager)
 

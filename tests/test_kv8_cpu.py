@@ -177,3 +177,20 @@ def test_definition_rounds_as_torch():
                    torch.tensor([0.0, -0.0, 448.0, 464.0, 1e9, -1e9])]).clamp(-448, 448)
     assert np.array_equal(ref.to_codes(x.numpy(), "fp8"),
                           x.to(torch.float8_e4m3fn).view(torch.uint8).numpy())
+
+
+def test_torch_ops_schemas_and_fakes(tq4):
+    ops = torch.ops.tq4
+    m = lambda *s, dtype=torch.int32: torch.empty(s, dtype=dtype, device="meta")  # noqa: E731
+    assert str(ops.paged_plan.default._schema).count("!") == 8
+    w = str(ops.kv8_reshape_and_cache.default._schema)
+    assert "Tensor(a2!) key_cache" in w and "Tensor(a4!) scale_cache" in w and w.endswith("-> ()")
+    c = (m(9, 2, 16, 64, dtype=torch.int8), m(9, 2, 1, 64, 16, dtype=torch.int8),
+         m(2, 9, 2, dtype=torch.float32))
+    q = m(7, 8, 64, dtype=torch.float16)
+    for out in (ops.kv8_paged_decode(q, *c, m(7, 3), m(7), 0, 0.0),
+                ops.kv8_paged_prefill(q, *c, m(2, 3), m(2), m(3), 4, True, 0.0)):
+        assert out.shape == q.shape and out.dtype == q.dtype and out.device.type == "meta"
+    with pytest.raises(NotImplementedError):
+        ops.kv8_paged_decode(*[torch.zeros(x.shape, dtype=x.dtype) for x in (q, *c, m(7, 3), m(7))],
+                             0, 0.0)
