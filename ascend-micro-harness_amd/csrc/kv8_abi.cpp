@@ -88,9 +88,23 @@ size_t record_bytes(const Cut& c, uint64_t items, uint32_t rec_rows, uint32_t d)
     return b > (uint64_t)SIZE_MAX - 16 ? SIZE_MAX : (size_t)((b + 15) & ~15ull);
 }
 
-// Whether the decode kernel takes a prefill call: row tiles of 16 that each read
-// the context, split over it, against tiles of 128 and more in LDS.
-bool few_rows(uint64_t rows) { return rows <= 64; }
+// Whether the decode kernel takes a prefill call: its tiles of 16 rows each read
+// the context from L2, and are as many workgroups more, against tiles of 128 rows
+// and more in LDS. Measured with 4 rows of 8 KV heads of 128 a token:
+//   32 rows   16 sequences of 500..4000 tokens  31 us for 42;  of 500..1000  10, 24
+//   512 rows  4 sequences of 1000 tokens        28 us for 42;  of 4000     107, 61
+//   256 rows  1 sequence of 4096                22 us for 36;  of 32768     83, 67
+// Up to 32 rows it is the better; behind, while its tiles times the tokens that a
+// table holds are few. One sequence is cut into even parts and takes twice that.
+bool few_rows(uint64_t num_rows, uint64_t seqs, uint64_t heads, uint64_t group, uint64_t max_q,
+              uint64_t cap)
+{
+    const uint64_t tiles = tiles_of(max_q, group);
+    if (tiles <= 2) return true;
+    uint64_t all = mul(seqs, tiles);
+    if (all > num_rows * group / tq4::kKv8Rows + seqs) all = num_rows * group / tq4::kKv8Rows + seqs;
+    return mul(heads, tiles) <= 65535u && mul(all, heads, cap) <= (seqs == 1 ? 2621440u : 1310720u);
+}
 
 // The parts that a prefill's row tiles cut their tokens into: with fewer row tiles
 // than the CUs hold at once, as many as fill them, of 256 tokens at least and while
@@ -318,14 +332,14 @@ size_t tq4_kv8_prefill_workspace_bytes(uint32_t num_rows, uint32_t num_seqs, uin
 {
     if (num_kv_heads == 0) return 0;
     if (max_query_len > num_rows) max_query_len = num_rows;
-    const uint64_t group = num_heads / num_kv_heads;
-    if (!few_rows(max_query_len * group)) {
+    const uint64_t group = num_heads / num_kv_heads, cap = (uint64_t)max_blocks_per_seq * block_size;
+    if (!few_rows(num_rows, num_seqs, num_kv_heads, group, max_query_len, cap)) {
         const uint32_t k = prefill_parts(head_size, num_rows, num_seqs, num_kv_heads, group,
-                                         max_query_len, (uint64_t)max_blocks_per_seq * block_size);
+                                         max_query_len, cap);
         return k == 1 ? 0 : record_bytes(Cut{k, 0, 0}, mul(num_rows, num_heads), 1, head_size);
     }
-    const Cut c = cut_rule(head_size, num_seqs, num_kv_heads, tiles_of(max_query_len, group),
-                           (uint64_t)max_blocks_per_seq * block_size, 0);
+    const Cut c =
+        cut_rule(head_size, num_seqs, num_kv_heads, tiles_of(max_query_len, group), cap, 0);
     return record_bytes(c, mul(num_seqs, num_kv_heads, tiles_of(max_query_len, group)),
                         record_rows(max_query_len, group), head_size);
 }
@@ -361,7 +375,7 @@ int tq4_kv8_paged_prefill(void* stream, int element_type, int code_type, const v
         tq4_kv8_prefill_workspace_bytes(num_rows, num_seqs, num_heads, num_kv_heads, head_size,
                                         block_size, max_blocks_per_seq, max_query_len);
     const bool room = !need || (workspace && aligned(workspace) && workspace_bytes >= need);
-    if (!few_rows(max_query_len * group)) {
+    if (!few_rows(num_rows, num_seqs, num_kv_heads, group, max_query_len, cap)) {
         const uint32_t k = prefill_parts(head_size, num_rows, num_seqs, num_kv_heads, group,
                                          max_query_len, cap);
         if (mul(mul(rows / 128 + num_seqs, num_kv_heads), k) > kMaxGroups / 2 ||

@@ -222,18 +222,23 @@ def check_prefill(tq4, q, c, lens, rows, code, causal, pad=0, tail=0, max_q=None
                                     1 / math.sqrt(d), max_q)
     dk, dv, ds, dt = on_device(kc, vc, sc, tables, code)
     qd = q.to(DEV)
-    out = torch.full(q.shape, 77.0, dtype=q.dtype, device=DEV)
-    print("prefill", tuple(q.shape), kc.shape, q.dtype, code, causal, list(lens)[:6],
-          list(rows)[:6], flush=True)
-    got = tq4.kv8_paged_prefill(wide(qd, pad) if pad else qd, dk, dv, ds, dt,
-                                dev(np.asarray(lens, np.int32)), dev(cu),
-                                max(rows, default=0) if max_q is None else max_q, causal=causal,
-                                out=out, **kw)
-    torch.cuda.synchronize()
-    assert got is out
-    assert (out[torch.from_numpy(~done).to(DEV)] == 77.0).all()
     at = torch.from_numpy(done)
-    print("of the bound:", ref.check(out[at.to(DEV)], want[done], off[done], q.dtype))
+    # a table of many pages more takes more than a few rows to the kernel for prompts
+    S = kc.shape[2]
+    far = torch.full((len(lens), max(900000 // S, dt.shape[1])), -1, dtype=torch.int32, device=DEV)
+    far[:, :dt.shape[1]] = dt
+    for t in (dt, far) if max(lens) <= dt.shape[1] * S else (dt,):
+        out = torch.full(q.shape, 77.0, dtype=q.dtype, device=DEV)
+        print("prefill", tuple(q.shape), kc.shape, tuple(t.shape), q.dtype, code, causal,
+              list(lens)[:6], list(rows)[:6], flush=True)
+        got = tq4.kv8_paged_prefill(wide(qd, pad) if pad else qd, dk, dv, ds, t,
+                                    dev(np.asarray(lens, np.int32)), dev(cu),
+                                    max(rows, default=0) if max_q is None else max_q,
+                                    causal=causal, out=out, **kw)
+        torch.cuda.synchronize()
+        assert got is out
+        assert (out[torch.from_numpy(~done).to(DEV)] == 77.0).all()
+        print("of the bound:", ref.check(out[at.to(DEV)], want[done], off[done], q.dtype))
     return out
 
 
@@ -279,6 +284,18 @@ def test_prefill_parts(tq4, d, G, rows, lens, causal):
     assert tq4.kv8_prefill_workspace_bytes(sum(rows), len(rows), G, 1, d, 32, c[3].shape[1],
                                            max(rows)) > 0
     check_prefill(tq4, queries(r, sum(rows) + 1, G, d, "fp16"), c, lens, rows, "int8", causal)
+
+
+@pytest.mark.parametrize("d,causal", [(64, True), (128, False), (256, True)])
+def test_prefill_of_many_rows(tq4, d, causal):
+    """Row tiles enough for the GPU: nothing is cut."""
+    r = np.random.default_rng(d)
+    lens, rows = [1000, 555, 33, 700], [900, 555, 1, 77]
+    H = 32 if d < 256 else 24
+    c = cache(r, lens, H, 16, d, "fp8")
+    assert tq4.kv8_prefill_workspace_bytes(sum(rows), 4, H, H, d, 16, c[3].shape[1],
+                                           max(rows)) == 0
+    check_prefill(tq4, queries(r, sum(rows) + 1, H, d, "bf16"), c, lens, rows, "fp8", causal)
 
 
 def test_prefill_wrong_lengths_stay_inside(tq4):
@@ -418,7 +435,7 @@ def test_captured_prefill(tq4):
     """Captured prefills, in parts and streamed, replayed with eager work between."""
     r = np.random.default_rng(23)
     lens, rows = [2100, 1500], [100, 30]
-    c = cache(r, lens, 1, 16, 128, "fp8")
+    c = cache(r, lens, 1, 16, 128, "fp8", width=6000)
     kc, vc, sc, tables = on_device(*c, "fp8")
     L = dev(np.array(lens, np.int32))
     for n in (rows, [3, 4]):
