@@ -51,24 +51,32 @@ uint64_t tiles_of(uint64_t max_q, uint64_t group)
     return (max_q * group + tq4::kKv8Rows - 1) / tq4::kKv8Rows;
 }
 
-// Tables of up to 1024 tokens are not worth a second kernel: one workgroup an
-// item. One sequence: even parts, of 256 tokens (a unit a wave) at least. Several:
-// streamed over as many workgroups as the CUs hold, at least four units each.
+// One workgroup an item needs no second kernel, and streaming (which keeps all CUs
+// busy whatever the lengths are) or parts save what it takes longer. A workgroup
+// walks cap tokens in cap * d * 0.0375 ns; all items together cost their bytes at
+// 4.9 TB/s. Within 4.5 us of that, and up to 20 us (contexts of unequal lengths), one
+// workgroup it is: heads of 128, 8 KV heads,
+//   16 sequences of 600..2048 tokens   13.2 us for 17.7 streamed
+//   32 of 500..4096                    35.8 for 38.6;  8 of 4096   22.1 for 17.6
+//   128 of 500..4096                   127 for 116 (even ones 190 for 212)
+// One sequence longer than 1024: even parts, of 256 tokens (a unit a wave) at least.
+// Several: streamed over as many workgroups as the CUs hold, four units each at least.
 Cut cut_rule(uint32_t d, uint64_t seqs, uint64_t heads, uint64_t tiles, uint64_t cap,
              uint32_t num_splits)
 {
     Cut c{num_splits, 0, 4};
     if (num_splits) return c;
     c.groups = 256u * (uint32_t)tq4::kKv8GroupsPerCu((int)d);
-    if (cap <= 1024) {
-        c.K = 1;
-    } else if (seqs == 1) {
-        const uint64_t items = heads * tiles ? heads * tiles : 1;
-        uint64_t k = c.groups / items;
+    const uint64_t items = mul(heads, tiles);
+    if (seqs == 1) {
+        uint64_t k = cap <= 1024 ? 1 : c.groups / (items ? items : 1);
         if (k > (cap + 255) / 256) k = (cap + 255) / 256;
         if (k > TQ4_KV8_MAX_SPLITS) k = TQ4_KV8_MAX_SPLITS;
         c.K = (uint32_t)(k ? k : 1);
+        return c;
     }
+    const uint64_t walk = mul(cap, d * 3ull) / 80, all = mul(mul(seqs, items), cap, d * 2ull) / 4900;
+    if (walk <= 20000 && walk <= all + 4500) c.K = 1;
     return c;
 }
 
@@ -90,20 +98,24 @@ size_t record_bytes(const Cut& c, uint64_t items, uint32_t rec_rows, uint32_t d)
 
 // Whether the decode kernel takes a prefill call: its tiles of 16 rows each read
 // the context from L2, and are as many workgroups more, against tiles of 128 rows
-// and more in LDS. Measured with 4 rows of 8 KV heads of 128 a token:
-//   32 rows   16 sequences of 500..4000 tokens  31 us for 42;  of 500..1000  10, 24
-//   512 rows  4 sequences of 1000 tokens        28 us for 42;  of 4000     107, 61
-//   256 rows  1 sequence of 4096                22 us for 36;  of 32768     83, 67
-// Up to 32 rows it is the better; behind, while its tiles times the tokens that a
-// table holds are few. One sequence is cut into even parts and takes twice that.
-bool few_rows(uint64_t num_rows, uint64_t seqs, uint64_t heads, uint64_t group, uint64_t max_q,
-              uint64_t cap)
+// and more in LDS. Up to 32 rows it is the better; behind, while its tiles are at
+// most three times those that the GPU holds at once, and its tiles times a table's
+// tokens are few. Measured with 4 rows of 8 KV heads of 128 a token (us, decode
+// kernel against the other):
+//   32 rows   16 sequences of 500..4000 tokens  32, 42;  of 500..1000   10, 24
+//   64 rows   the same                          43, 48;  256 rows of 500..4000  105, 107
+//   512 rows  4 sequences of 1000 tokens        28, 42;  1024 rows      48, 45
+//   256 rows  1 sequence of 4096                22, 36;  512 rows of 32768     156, 97
+bool few_rows(uint32_t d, uint64_t num_rows, uint64_t seqs, uint64_t heads, uint64_t group,
+              uint64_t max_q, uint64_t cap)
 {
     const uint64_t tiles = tiles_of(max_q, group);
     if (tiles <= 2) return true;
     uint64_t all = mul(seqs, tiles);
     if (all > num_rows * group / tq4::kKv8Rows + seqs) all = num_rows * group / tq4::kKv8Rows + seqs;
-    return mul(heads, tiles) <= 65535u && mul(all, heads, cap) <= (seqs == 1 ? 2621440u : 1310720u);
+    all = mul(all, heads);
+    return mul(heads, tiles) <= 65535u && all <= 768ull * tq4::kKv8GroupsPerCu((int)d) &&
+           mul(all, cap) <= (d == 256 && seqs > 1 ? 1310720u : 2250000u);
 }
 
 // The parts that a prefill's row tiles cut their tokens into: with fewer row tiles
@@ -333,7 +345,7 @@ size_t tq4_kv8_prefill_workspace_bytes(uint32_t num_rows, uint32_t num_seqs, uin
     if (num_kv_heads == 0) return 0;
     if (max_query_len > num_rows) max_query_len = num_rows;
     const uint64_t group = num_heads / num_kv_heads, cap = (uint64_t)max_blocks_per_seq * block_size;
-    if (!few_rows(num_rows, num_seqs, num_kv_heads, group, max_query_len, cap)) {
+    if (!few_rows(head_size, num_rows, num_seqs, num_kv_heads, group, max_query_len, cap)) {
         const uint32_t k = prefill_parts(head_size, num_rows, num_seqs, num_kv_heads, group,
                                          max_query_len, cap);
         return k == 1 ? 0 : record_bytes(Cut{k, 0, 0}, mul(num_rows, num_heads), 1, head_size);
@@ -375,7 +387,7 @@ int tq4_kv8_paged_prefill(void* stream, int element_type, int code_type, const v
         tq4_kv8_prefill_workspace_bytes(num_rows, num_seqs, num_heads, num_kv_heads, head_size,
                                         block_size, max_blocks_per_seq, max_query_len);
     const bool room = !need || (workspace && aligned(workspace) && workspace_bytes >= need);
-    if (!few_rows(num_rows, num_seqs, num_kv_heads, group, max_query_len, cap)) {
+    if (!few_rows(head_size, num_rows, num_seqs, num_kv_heads, group, max_query_len, cap)) {
         const uint32_t k = prefill_parts(head_size, num_rows, num_seqs, num_kv_heads, group,
                                          max_query_len, cap);
         if (mul(mul(rows / 128 + num_seqs, num_kv_heads), k) > kMaxGroups / 2 ||
