@@ -474,7 +474,6 @@ __global__ __launch_bounds__(kThreads, kKv8GroupsPerCu(D)) void kv8_decode(Kv8At
         return true;
     };
 
-    const uint32_t step = kWaves * kUnit;
     for (;;) {
         Sums<D> sums;
 #pragma unroll

@@ -54,7 +54,11 @@ __device__ __forceinline__ float widen_el(uint32_t bits16)
 template <int BF16>
 __device__ __forceinline__ uint32_t narrow2(float a, float b)
 {
-    if constexpr (BF16) return f32_to_bf16(a) | f32_to_bf16(b) << 16;
+    if constexpr (BF16) {
+        typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+        const b2_t h = {(__bf16)a, (__bf16)b};  // v_cvt_pk_bf16_f32
+        return __builtin_bit_cast(uint32_t, h);
+    }
     const h2_t h = {(_Float16)a, (_Float16)b};
     return __builtin_bit_cast(uint32_t, h);
 }
