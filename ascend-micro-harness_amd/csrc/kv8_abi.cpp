@@ -126,7 +126,7 @@ bool few_rows(uint32_t d, uint64_t num_rows, uint64_t seqs, uint64_t heads, uint
 uint32_t prefill_parts(uint32_t d, uint64_t num_rows, uint64_t seqs, uint64_t heads,
                        uint64_t group, uint64_t max_q, uint64_t cap)
 {
-    const uint64_t waves = tq4::kv8_prefill_waves(d, max_q * group), rows = 32 * waves;
+    const uint64_t waves = tq4::kv8_prefill_waves(d, max_q * group, cap), rows = 32 * waves;
     uint64_t tiles = mul(seqs, (max_q * group + rows - 1) / rows);
     if (tiles > mul(num_rows, group) / rows + seqs) tiles = mul(num_rows, group) / rows + seqs;
     const uint64_t groups = mul(tiles, heads);

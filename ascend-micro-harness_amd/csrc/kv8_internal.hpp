@@ -53,11 +53,15 @@ struct Kv8AttnParams {
     float scale;
 };
 // Waves of a prefill workgroup, 32 rows each (kv8_prefill.hip), for so many rows of
-// a (sequence, kv head), and the workgroups that the CUs hold at once. Eight waves
-// widen a tile for twice the rows (8192 rows x 32 heads of 128: 619 us against 651);
-// heads of 64 run better as three workgroups of four a CU (418 against 376 us), and
+// a (sequence, kv head) over tables of `cap` tokens, and the workgroups that the CUs
+// hold at once. Eight waves widen a tile for twice the rows (8192 rows x 32 heads of
+// 128: 619 us against 651), four are the more balanced where there are few tiles
+// (2048 rows: 72 us against 81; 1000: 37, 42); heads of 64 run better as three workgroups of four a CU (418 against 376 us), and
 // 256 channels fill a wave's registers and a CU's LDS with four.
-inline uint32_t kv8_prefill_waves(uint32_t d, uint64_t rows) { return d == 128 && rows > 128 ? 8 : 4; }
+inline uint32_t kv8_prefill_waves(uint32_t d, uint64_t rows, uint64_t cap)
+{
+    return d == 128 && rows > 128 && cap > 2048 ? 8 : 4;
+}
 inline uint32_t kv8_prefill_fit(uint32_t d, uint32_t waves)
 {
     return 256u * (waves == 8 || d == 256 ? 1 : d == 128 ? 2 : 3);

@@ -470,7 +470,7 @@ template <int D, int BF16, int INT8>
 hipError_t launch_w(hipStream_t stream, const Kv8AttnParams& p)
 {
     if constexpr (D == 128) {
-        if (kv8_prefill_waves(D, (uint64_t)p.max_q * p.G) == 8)
+        if (kv8_prefill_waves(D, (uint64_t)p.max_q * p.G, (uint64_t)p.M * p.S) == 8)
             return launch_t<D, BF16, INT8, 8>(stream, p);
     }
     return launch_t<D, BF16, INT8, 4>(stream, p);
