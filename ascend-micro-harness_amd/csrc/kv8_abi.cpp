@@ -51,32 +51,40 @@ uint64_t tiles_of(uint64_t max_q, uint64_t group)
     return (max_q * group + tq4::kKv8Rows - 1) / tq4::kKv8Rows;
 }
 
-// One workgroup an item needs no second kernel, and streaming (which keeps all CUs
-// busy whatever the lengths are) or parts save what it takes longer. A workgroup
-// walks cap tokens in cap * d * 0.0375 ns; all items together cost their bytes at
-// 4.9 TB/s. Within 4.5 us of that, and up to 20 us (contexts of unequal lengths), one
-// workgroup it is: heads of 128, 8 KV heads,
-//   16 sequences of 600..2048 tokens   13.2 us for 17.7 streamed
-//   32 of 500..4096                    35.8 for 38.6;  8 of 4096   22.1 for 17.6
-//   128 of 500..4096                   127 for 116 (even ones 190 for 212)
-// One sequence longer than 1024: even parts, of 256 tokens (a unit a wave) at least.
-// Several: streamed over as many workgroups as the CUs hold, four units each at least.
+// The choice between one workgroup an item (no second kernel), even parts, and
+// streaming, which keeps all CUs busy whatever the lengths are. A workgroup walks cap
+// tokens in cap * d * 0.0375 ns, all items together cost their bytes at 4.9 TB/s
+// (3.9 with half the CUs) and a second kernel 4 us. Heads of 128, 8 KV heads, us for
+// one workgroup / parts / streamed:
+//   4 sequences of 300..1500 tokens   10.8 /  8.5 / 11.0   parts: one workgroup a CU
+//   16 of 300..1500                   10.8 / 12.6 / 17.7
+//   16 of 300..4099                   22.5 / 19.2 / 25.7
+//   16 of 500..20000                  128  / 84   / 72     parts of 10000: uneven
+//   32 of 500..4096                   35.8 / 41.5 / 38.6
+//   128 of 500..4096                  127  / 125  / 116    (even ones 190 / 211 / 212)
+// One sequence longer than 1024: parts for all workgroups that the CUs hold. Parts
+// have 256 tokens (a unit a wave) at least, a streamed workgroup four units.
 Cut cut_rule(uint32_t d, uint64_t seqs, uint64_t heads, uint64_t tiles, uint64_t cap,
              uint32_t num_splits)
 {
     Cut c{num_splits, 0, 4};
     if (num_splits) return c;
     c.groups = 256u * (uint32_t)tq4::kKv8GroupsPerCu((int)d);
-    const uint64_t items = mul(heads, tiles);
+    uint64_t items = mul(seqs, heads, tiles);
+    if (items == 0) items = 1;
+    const uint64_t walk = mul(cap, d * 3ull) / 80, all = mul(mul(items, cap), d * 2ull) / 4900;
+    uint64_t k = seqs == 1 ? (cap <= 1024 ? 1 : c.groups / items) : 256 / items;
+    if (k > (cap + 255) / 256) k = (cap + 255) / 256;
+    if (k > TQ4_KV8_MAX_SPLITS) k = TQ4_KV8_MAX_SPLITS;
     if (seqs == 1) {
-        uint64_t k = cap <= 1024 ? 1 : c.groups / (items ? items : 1);
-        if (k > (cap + 255) / 256) k = (cap + 255) / 256;
-        if (k > TQ4_KV8_MAX_SPLITS) k = TQ4_KV8_MAX_SPLITS;
         c.K = (uint32_t)(k ? k : 1);
-        return c;
+    } else if (k > 1) {
+        const uint64_t one = walk > all / 4 * 5 ? walk : all / 4 * 5;
+        const uint64_t parts = (walk / k > all ? walk / k : all) + 4000;
+        c.K = one <= parts ? 1 : walk / k <= 15000 ? (uint32_t)k : 0;
+    } else if (walk <= 20000 && walk <= all + 4500) {
+        c.K = 1;
     }
-    const uint64_t walk = mul(cap, d * 3ull) / 80, all = mul(mul(seqs, items), cap, d * 2ull) / 4900;
-    if (walk <= 20000 && walk <= all + 4500) c.K = 1;
     return c;
 }
 
