@@ -219,13 +219,14 @@ def test_decode_offsets_past_32_bits(tq4):
 
 
 # ------------------------------------------------------------ several rows
-def check_prefill(tq4, q, c, lens, rows, code, causal, pad=0, tail=0, max_q=None, **kw):
-    """`tail` rows behind the last sequence, which have to stay as they were."""
+def check_prefill(tq4, q, c, lens, rows, code, causal, pad=0, max_q=None, scale=None, **kw):
+    """Rows behind the last sequence have to stay as they were."""
     kc, vc, sc, tables = c
     d = q.shape[2]
     cu = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
     want, off, done = ref.attention(q.double().numpy(), kc, vc, sc, tables, lens, cu, code, causal,
-                                    1 / math.sqrt(d), max_q)
+                                    1 / math.sqrt(d) if scale is None else scale, max_q)
+    kw["scale"] = scale
     dk, dv, ds, dt = on_device(kc, vc, sc, tables, code)
     qd = q.to(DEV)
     at = torch.from_numpy(done)
@@ -331,6 +332,37 @@ def test_prefill_scales_far_apart(tq4, code):
             sc[0, p] = 2.0 ** -9 * 1.2 ** i
             sc[1, p] = 2.0 ** (-9 - i % 7)
     check_prefill(tq4, queries(r, 483, 4, 128, "fp16"), c, lens, rows, code, True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_prefill_queries_of_every_size(tq4, dtype):
+    """Scales that are negative, zero or large; rows of zeros, of tiny and huge
+    magnitude; a row with a NaN or an infinity is its own affair."""
+    r = np.random.default_rng(14)
+    lens, rows = [300, 129], [120, 40]
+    for d in (64, 128, 256):
+        c = cache(r, lens, 1, 16, d, "fp8", spread=1)
+        q = queries(r, 160, 4, d, dtype).double()
+        q[7] = 0
+        q[8] *= 2.0 ** -12 if dtype == "fp16" else 2.0 ** -120
+        q[9] *= 2.0 ** 9 if dtype == "fp16" else 2.0 ** 20
+        q = q.to(ref.TYPES[dtype])
+        for scale in (-0.2, 0.0, 1.0):
+            check_prefill(tq4, q, c, lens, rows, "fp8", True, scale=scale)
+        kc, vc, sc, t = on_device(*c, "fp8")
+        L, cu = dev(np.array(lens, np.int32)), dev(np.array([0, 120, 160], np.int32))
+        far = torch.full((2, 50000), -1, dtype=torch.int32, device=DEV)
+        far[:, :t.shape[1]] = t
+        bad = q.clone()
+        bad[3, 1, 5], bad[130, 2, 0] = float("nan"), float("inf")
+        keep = torch.ones(160, 4, dtype=torch.bool)
+        keep[3, 1] = keep[130, 2] = False
+        for table in (t, far):
+            print("bad rows", d, tuple(table.shape), flush=True)
+            fine = tq4.kv8_paged_prefill(q.to(DEV), kc, vc, sc, table, L, cu, 120)
+            out = tq4.kv8_paged_prefill(bad.to(DEV), kc, vc, sc, table, L, cu, 120)
+            assert torch.equal(out.cpu()[keep], fine.cpu()[keep])
+            assert out[3, 1].isnan().all()
 
 
 # ------------------------------------------------------------- a step of all
