@@ -291,16 +291,29 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
         }
         if (t0 >= some) continue;
 
+        // The tile's operand blocks in the order of their MFMA: the keys of both
+        // blocks of tokens, then the values strip by strip. A ring of registers
+        // holds the next kRing of them, or each MFMA would wait for its LDS read.
+        constexpr int kRing = 4, kScores = 2 * KK;
+        h8_t ring[kRing];
+        auto operand = [&](int i) {
+            const int to = i < kScores ? i * Tile<D>::kKeyBlock
+                                       : Tile<D>::kKeys + (i - kScores) * 1024;
+            return *(const h8_t*)(tile + to + lane * 16);
+        };
         f16_t s[2];
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb) {
+        for (int i = 0; i < kRing; ++i) ring[i] = operand(i);
+        __builtin_amdgcn_sched_group_barrier(0x100, kRing, 0);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[tb][i] = 0.0f;
+        for (int i = 0; i < 16; ++i) s[0][i] = s[1][i] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < KK; ++k)
-                s[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                    *(const h8_t*)(tile + (tb * KK + k) * Tile<D>::kKeyBlock + lane * 16), q[k],
-                    s[tb], 0, 0, 0);
+        for (int i = 0; i < kScores; ++i) {
+            s[i / KK] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % kRing], q[i % KK], s[i / KK],
+                                                               0, 0, 0);
+            ring[i % kRing] = operand(i + kRing);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         StripInfo st[kStrips];
         int least = 16;
@@ -356,12 +369,11 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
             l += sum * st[x].rvs;
         }
 #pragma unroll
-        for (int c = 0; c < CB; ++c)
-#pragma unroll
-            for (int x = 0; x < kStrips; ++x)
-                o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                    *(const h8_t*)(tile + Tile<D>::kKeys + (x * CB + c) * 1024 + lane * 16), pr[x],
-                    o[c], 0, 0, 0);
+        for (int i = 0; i < kScores; ++i) {
+            const int c = i % CB;
+            o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % kRing], pr[i / CB], o[c], 0, 0, 0);
+            if (i + kRing < kScores) ring[i % kRing] = operand(kScores + i + kRing);
+        }
     }
 
     const uint32_t row = seq.row0 + f / p.G;
