@@ -10,10 +10,14 @@
 // however often the scale grew (half a step each time, of a step that doubles).
 //
 // Runs of several rows (prompts) go to waves a strip of 16 offsets each, up to
-// four waves a page, which exchange their amax; an LDS map from the page's offsets
+// eight waves a page, which exchange their amax; an LDS map from the page's offsets
 // to rows puts any order of rows, and repeats, right. Single rows (a decode step)
 // go to 16 lanes each. Waves find their runs themselves, from the slots of a window
 // of rows and its neighbours.
+//
+// Memory bounds the prompts: 16384 rows of 8 heads of 128 24.3 us, 4.1 TB/s of the
+// 4.9 that a copy reaches (a wave a whole page: 34 us, its strips one after the
+// other). 64 single rows 3.7 us, a launch; a wave a row instead of 16 lanes 6.0.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
