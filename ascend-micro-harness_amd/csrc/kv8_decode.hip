@@ -513,12 +513,12 @@ __global__ __launch_bounds__(TEAM > kWaves ? 64 * TEAM : kThreads) void kv8_comb
     if (row < s.row0 || row - s.row0 >= s.rows) return;
     const uint32_t f = (row - s.row0) * p.G + hq % p.G, h = hq / p.G;
     const uint32_t rt = f / kRows, r = f % kRows;
-    // its records: K of them, the first at slot0, the others from `slot` on
-    uint32_t K, apart;
+    // its records: at most `bound` of them, the first at slot0, the others from
+    // `slot` on
+    uint32_t bound, apart;
     uint64_t slot0, slot;
     if (p.K) {
-        const uint32_t w = part_units(p, s.units());
-        K = (s.units() + w - 1) / w;
+        bound = p.K;
         slot0 = (((uint64_t)b * p.Hkv + h) * max_tiles + rt) * p.K;
         slot = slot0 + 1;
         apart = 1;
@@ -533,15 +533,22 @@ __global__ __launch_bounds__(TEAM > kWaves ? 64 * TEAM : kThreads) void kv8_comb
         const uint32_t quota = quota_of(p, total);
         const uint32_t from = before + (h * s.tiles(p) + rt) * s.units();
         const uint32_t w0 = from / quota, w1 = (from + s.units() - 1) / quota;
-        K = w1 - w0 + 1;
+        bound = w1 - w0 + 1;
         slot0 = 2ull * w0 + 1;
         slot = 2ull * w0 + 2;
         apart = 2;
     }
-    if (K < 2) return;  // the whole item went to the output
-    join_records<D, BF16, TEAM>(p, at, K, part, [&](uint32_t k) {
-        return (k ? slot + (uint64_t)(k - 1) * apart : slot0) * p.rec_rows + r;
-    });
+    if (bound < 2) return;  // the whole item went to the output
+    join_records<D, BF16, TEAM>(
+        p, at, bound, part,
+        [&](uint32_t k) {
+            return (k ? slot + (uint64_t)(k - 1) * apart : slot0) * p.rec_rows + r;
+        },
+        [&] {
+            if (p.K == 0) return bound;
+            const uint32_t w = part_units(p, s.units());
+            return (s.units() + w - 1) / w;
+        });
 }
 
 template <int D, int BF16, int INT8>

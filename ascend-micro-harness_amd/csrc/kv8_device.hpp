@@ -173,38 +173,53 @@ __device__ __forceinline__ uint32_t sequence_of(const Kv8AttnParams& p, uint32_t
     return lo;
 }
 
-// The K records of output row `at`, weights 2^(m_k - max m), to the output. TEAM
-// waves take them in turn and merge in `part` (TEAM rows; one wave: not used);
-// record(k): the index of record k.
-template <int D, int BF16, int TEAM, class Record>
-__device__ __forceinline__ void join_records(const Kv8AttnParams& p, uint64_t at, uint32_t K,
-                                             float (*part)[D], Record&& record)
+// The records of output row `at`, weights 2^(m_k - max m), to the output. TEAM
+// waves take them in turn and merge in `part` (TEAM rows; one wave: not used).
+// record(k): the index of record k < bound; count(): how many of them were written,
+// fewer than 2 where the row is none of the join's. The first loads do not wait for
+// it: what they find past it is left out.
+template <int D, int BF16, int TEAM, class Record, class Count>
+__device__ __forceinline__ void join_records(const Kv8AttnParams& p, uint64_t at, uint32_t bound,
+                                             float (*part)[D], Record&& record, Count&& count)
 {
     constexpr int C = D / 64;
     const uint32_t lane = threadIdx.x & 63u, mine = (threadIdx.x >> 6) % TEAM;
-    float m = kNone;
-    for (uint32_t k = lane; k < K; k += 64) m = fmaxf(m, p.ml[2 * record(k)]);
+    float x[8][C];
+    // eight of the wave's records from k on (past the last: the last again)
+    auto load = [&](uint32_t k0, uint32_t k, uint32_t last) {
 #pragma unroll
-    for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, xor_lanes(m, i));
-    float a[C] = {}, l = 0.0f;
-    for (uint32_t k0 = 0; k0 < K; k0 += 64) {
-        float w = 0.0f;  // of record k0 + lane
-        if (k0 + lane < K) {
-            const float2 x = *(const float2*)(p.ml + 2 * record(k0 + lane));
-            w = __builtin_amdgcn_exp2f(x.x - m);
-            l += w * x.y;
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t kj = k0 + k + j * TEAM < last ? k0 + k + j * TEAM : last;
+            __builtin_memcpy(
+                x[j], __builtin_assume_aligned(p.acc + record(kj) * D + lane * C, 4 * C), 4 * C);
         }
-        // eight records' loads at a time (past the last: its sums again, weight 0)
+    };
+    auto stat = [&](uint32_t k) {
+        return k < bound ? *(const float2*)(p.ml + 2 * record(k)) : float2{kNone, 0.0f};
+    };
+    float2 st = stat(lane);
+    load(0, mine, bound - 1);
+    const uint32_t K = count();
+    if (K < 2) return;
+    float m = kNone, a[C] = {}, l = 0.0f;
+    for (uint32_t k0 = 0; k0 < K; k0 += 64) {
+        if (k0) {
+            st = stat(k0 + lane);
+            load(k0, mine, K - 1);
+        }
+        const bool held = k0 + lane < K;
+        float to = held ? fmaxf(m, st.x) : m;
+#pragma unroll
+        for (int i = 1; i < 64; i <<= 1) to = fmaxf(to, xor_lanes(to, i));
+        const float r = __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        const float w = held ? __builtin_amdgcn_exp2f(st.x - m) : 0.0f;  // of record k0 + lane
+        l = held ? l * r + w * st.y : l * r;
+#pragma unroll
+        for (int i = 0; i < C; ++i) a[i] *= r;
         const uint32_t n = K - k0 < 64 ? K - k0 : 64u;
         for (uint32_t k = mine; k < n; k += 8 * TEAM) {
-            float x[8][C];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t kj = k + j * TEAM < n ? k + j * TEAM : n - 1;
-                __builtin_memcpy(
-                    x[j], __builtin_assume_aligned(p.acc + record(k0 + kj) * D + lane * C, 4 * C),
-                    4 * C);
-            }
+            if (k != mine) load(k0, k, K - 1);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const bool in = k + j * TEAM < n;
