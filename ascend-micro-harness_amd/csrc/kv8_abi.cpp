@@ -56,14 +56,16 @@ uint64_t tiles_of(uint64_t max_q, uint64_t group)
 // tokens in cap * d * 0.0375 ns, all items together cost their bytes at 4.9 TB/s
 // (3.9 with half the CUs) and a second kernel 4 us. Heads of 128, 8 KV heads, us for
 // one workgroup / parts / streamed:
-//   4 sequences of 300..1500 tokens   10.8 /  8.5 / 11.0   parts: one workgroup a CU
+//   4 sequences of 300..1500 tokens   10.8 /  8.5 / 11.0
 //   16 of 300..1500                   10.8 / 12.6 / 17.7
 //   16 of 300..4099                   22.5 / 19.2 / 25.7
 //   16 of 500..20000                  128  / 84   / 72     parts of 10000: uneven
 //   32 of 500..4096                   35.8 / 41.5 / 38.6
 //   128 of 500..4096                  127  / 125  / 116    (even ones 190 / 211 / 212)
-// One sequence longer than 1024: parts for all workgroups that the CUs hold. Parts
-// have 256 tokens (a unit a wave) at least, a streamed workgroup four units.
+// Parts: one workgroup a CU (one sequence of 4096: 16 / 32 / 64 parts 8.5 / 7.8 / 8.7
+// us; of 65536 32 / 64 29.4 / 30.5), of 128 tokens at least, and no more than 64, or
+// 128, where the join's share grows (2 heads of 65536: 64 / 128 parts 12.8 / 13.3; of
+// 256 channels 20.8 / 19.1). A streamed workgroup has four units at least.
 Cut cut_rule(uint32_t d, uint64_t seqs, uint64_t heads, uint64_t tiles, uint64_t cap,
              uint32_t num_splits)
 {
@@ -73,16 +75,14 @@ Cut cut_rule(uint32_t d, uint64_t seqs, uint64_t heads, uint64_t tiles, uint64_t
     uint64_t items = mul(seqs, heads, tiles);
     if (items == 0) items = 1;
     const uint64_t walk = mul(cap, d * 3ull) / 80, all = mul(mul(items, cap), d * 2ull) / 4900;
-    uint64_t k = seqs == 1 ? (cap <= 1024 ? 1 : c.groups / items) : 256 / items;
-    if (k > (cap + 255) / 256) k = (cap + 255) / 256;
-    if (k > TQ4_KV8_MAX_SPLITS) k = TQ4_KV8_MAX_SPLITS;
-    if (seqs == 1) {
-        c.K = (uint32_t)(k ? k : 1);
-    } else if (k > 1) {
+    uint64_t k = 256 / items;
+    if (k > (cap + 127) / 128) k = (cap + 127) / 128;
+    if (k > (d == 256 ? 128 : 64)) k = d == 256 ? 128 : 64;
+    if (k > 1) {
         const uint64_t one = walk > all / 4 * 5 ? walk : all / 4 * 5;
         const uint64_t parts = (walk / k > all ? walk / k : all) + 4000;
-        c.K = one <= parts ? 1 : walk / k <= 15000 ? (uint32_t)k : 0;
-    } else if (walk <= 20000 && walk <= all + 4500) {
+        c.K = one <= parts ? 1 : seqs == 1 || walk / k <= 15000 ? (uint32_t)k : 0;
+    } else if (seqs == 1 || (walk <= 20000 && walk <= all + 4500)) {
         c.K = 1;
     }
     return c;
