@@ -14,6 +14,7 @@
 // The GIL is released around the launch, as ctypes does.
 #include <ATen/ATen.h>
 #include <Python.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
@@ -659,10 +660,21 @@ PyObject* entry8(PyObject* const* a, Py_ssize_t n, F&& f)
     });
 }
 
-at::Tensor bytes_like(const at::Tensor* t, size_t n)
-{
-    return at::empty({(int64_t)n}, t->options().dtype(at::kByte));
-}
+// A call's workspace: the caller's, or the call's own from torch's allocator, on the
+// current stream as a tensor's would be (without the tensor, 1 us of host time).
+struct Room {
+    c10::DataPtr own;
+    void* at;
+    size_t bytes;
+
+    template <class Need>
+    Room(const at::Tensor* given, Need&& need) : at(ptr(given)), bytes(nbytes(given))
+    {
+        if (given || (bytes = need()) == 0) return;
+        own = c10::hip::HIPCachingAllocator::get()->allocate(bytes);
+        at = own.get();
+    }
+};
 
 // A cache's sizes and its three tensors (kv8.py _pool).
 struct Pool8 {
@@ -713,18 +725,14 @@ PyObject* paged_plan(PyObject*, PyObject* const* a, Py_ssize_t n)
                     (!pos || holds_all(pos, slots->numel())) && (!ncl || holds_all(ncl, B)) &&
                     (!nstate || holds_all(nstate, 2))))
             return nullptr;
-        at::Tensor fresh;
-        if (!ws) {
-            fresh = bytes_like(bt, g_abi.paged_plan_workspace_bytes((uint32_t)B));
-            ws = &fresh;
-        }
+        const Room room(ws, [&] { return g_abi.paged_plan_workspace_bytes((uint32_t)B); });
         return PyLong_FromLong(unlocked([&] {
             return g_abi.paged_plan(
                 st, (const int32_t*)ptr(cl), (const int32_t*)ptr(ql), (const int32_t*)ptr(release),
                 (int32_t*)ptr(bt), (int32_t*)ptr(ring), (const int32_t*)ptr(state),
                 (int32_t*)ptr(slots), (int32_t*)ptr(pos), (int32_t*)ptr(cu),
                 (int32_t*)ptr(granted), (int32_t*)ptr(ncl ? ncl : cl),
-                (int32_t*)ptr(nstate ? nstate : state), ptr(ws), nbytes(ws), (uint32_t)B,
+                (int32_t*)ptr(nstate ? nstate : state), room.at, room.bytes, (uint32_t)B,
                 (uint32_t)bt->size(1), S, (uint32_t)ring->numel(), (uint32_t)slots->numel());
         }));
     });
@@ -816,21 +824,16 @@ PyObject* kv8_paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n)
         void* st = g.current_stream();
         if (!g.need(x.s.a == x.B && K <= TQ4_KV8_MAX_SPLITS && small(x.s.b))) return nullptr;
         const uint32_t Hq = (uint32_t)x.s.b;
-        at::Tensor made, room;
+        at::Tensor made;
         out.make(x, made);
-        if (!ws) {
-            const size_t need = g_abi.kv8_decode_workspace_bytes(x.B, Hq, x.c.H, x.c.d, x.c.S,
-                                                                 x.M, K);
-            if (need) {
-                room = bytes_like(x.q, need);
-                ws = &room;
-            }
-        }
+        const Room room(ws, [&] {
+            return g_abi.kv8_decode_workspace_bytes(x.B, Hq, x.c.H, x.c.d, x.c.S, x.M, K);
+        });
         const int rc = unlocked([&] {
             return g_abi.kv8_paged_decode(
                 st, x.element(), x.c.code, ptr(x.q), ptr(x.c.kc), ptr(x.c.vc),
                 (const float*)ptr(x.c.sc), (const int32_t*)ptr(x.bt), (const int32_t*)ptr(x.cl),
-                ptr(ws), nbytes(ws), ptr(out.t), x.stride, x.B, Hq, x.c.H, x.c.d, x.c.S, x.c.P,
+                room.at, room.bytes, ptr(out.t), x.stride, x.B, Hq, x.c.H, x.c.d, x.c.S, x.c.P,
                 x.M, K, scale);
         });
         return out.result(rc, made);
@@ -853,21 +856,16 @@ PyObject* kv8_paged_prefill(PyObject*, PyObject* const* a, Py_ssize_t n)
         void* st = g.current_stream();
         if (!g.need(holds_all(cu, (int64_t)x.B + 1))) return nullptr;
         const uint32_t Hq = (uint32_t)x.s.b, T = (uint32_t)x.s.a;
-        at::Tensor made, room;
+        at::Tensor made;
         out.make(x, made);
-        if (!ws) {
-            const size_t need = g_abi.kv8_prefill_workspace_bytes(T, x.B, Hq, x.c.H, x.c.d, x.c.S,
-                                                                  x.M, longest);
-            if (need) {
-                room = bytes_like(x.q, need);
-                ws = &room;
-            }
-        }
+        const Room room(ws, [&] {
+            return g_abi.kv8_prefill_workspace_bytes(T, x.B, Hq, x.c.H, x.c.d, x.c.S, x.M, longest);
+        });
         const int rc = unlocked([&] {
             return g_abi.kv8_paged_prefill(
                 st, x.element(), x.c.code, ptr(x.q), ptr(x.c.kc), ptr(x.c.vc),
                 (const float*)ptr(x.c.sc), (const int32_t*)ptr(x.bt), (const int32_t*)ptr(x.cl),
-                (const int32_t*)ptr(cu), ptr(ws), nbytes(ws), ptr(out.t), x.stride, T, x.B, Hq,
+                (const int32_t*)ptr(cu), room.at, room.bytes, ptr(out.t), x.stride, T, x.B, Hq,
                 x.c.H, x.c.d, x.c.S, x.c.P, x.M, longest, causal, scale);
         });
         return out.result(rc, made);
