@@ -146,9 +146,12 @@ uint32_t prefill_parts(uint32_t d, uint64_t num_rows, uint64_t seqs, uint64_t he
     return (uint32_t)(k < 1 ? 1 : k > 64 ? 64 : k);
 }
 
-// The grid and the line of a streamed call's units in bounds.
-bool cut_fits(const Cut& c, uint64_t seqs, uint64_t cap, uint64_t heads, uint64_t tiles)
+// The grids and the line of a streamed call's units in bounds; `rows` output rows,
+// each a workgroup of the join, of 1024 where there are many records.
+bool cut_fits(const Cut& c, uint64_t seqs, uint64_t cap, uint64_t heads, uint64_t tiles,
+              uint64_t rows)
 {
+    if (rows > (c.K > 32 ? kMaxGroups / 4 : kMaxGroups)) return false;
     if (c.K) return mul(seqs, c.K) <= kMaxGroups && mul(heads, tiles) <= 65535u;
     return mul(mul(seqs, (cap + tq4::kKv8Unit - 1) / tq4::kKv8Unit), heads, tiles) <= 0xff000000ull;
 }
@@ -332,7 +335,7 @@ int tq4_kv8_paged_decode(void* stream, int element_type, int code_type, const vo
     if (num_splits > TQ4_KV8_MAX_SPLITS) return TQ4_ERR_SPLITS;
     const uint64_t cap = (uint64_t)max_blocks_per_seq * block_size;
     const Cut s = cut_rule(head_size, num_seqs, num_kv_heads, 1, cap, num_splits);
-    if (!cut_fits(s, num_seqs, cap, num_kv_heads, 1) || mul(num_seqs, num_heads) > kMaxGroups)
+    if (!cut_fits(s, num_seqs, cap, num_kv_heads, 1, mul(num_seqs, num_heads)))
         return TQ4_ERR_RANGE;
     const size_t need = tq4_kv8_decode_workspace_bytes(num_seqs, num_heads, num_kv_heads, head_size,
                                                        block_size, max_blocks_per_seq, num_splits);
@@ -408,7 +411,7 @@ int tq4_kv8_paged_prefill(void* stream, int element_type, int code_type, const v
                                                 code_type == TQ4_KV8_INT8, p));
     }
     const Cut s = cut_rule(head_size, num_seqs, num_kv_heads, tiles, cap, 0);
-    if (!cut_fits(s, num_seqs, cap, num_kv_heads, tiles) || mul(num_rows, num_heads) > kMaxGroups)
+    if (!cut_fits(s, num_seqs, cap, num_kv_heads, tiles, mul(num_rows, num_heads)))
         return TQ4_ERR_RANGE;
     if (!room) return TQ4_ERR_WORKSPACE;
     return launched(tq4::launch_kv8_decode((hipStream_t)stream, element_type,

@@ -319,6 +319,69 @@ def test_prefill_wrong_lengths_stay_inside(tq4):
     check_prefill(tq4, q, c, [200, 90, 10 ** 6], rows, "fp8", True, max_q=3)
 
 
+def test_prefill_row_ranges(tq4):
+    """Rows before the first sequence and past num_rows, ranges without rows."""
+    r = np.random.default_rng(15)
+    lens, cu = [300, 50, 120, 90], np.array([7, 60, 60, 180, 200], np.int32)
+    for d, H in ((64, 1), (128, 2), (256, 1)):
+        c = cache(r, lens, H, 16, d, "int8")
+        kc, vc, sc, t = on_device(*c, "int8")
+        far = torch.full((4, 60000), -1, dtype=torch.int32, device=DEV)
+        far[:, :t.shape[1]] = t
+        q = queries(r, 200, 4 * H, d, "bf16")
+        want, off, done = ref.attention(q.double().numpy(), *c, lens, cu, "int8", True,
+                                        1 / math.sqrt(d))
+        for rows in (200, 150, 60, 8, 7):
+            for table in (t, far):
+                print("ranges", d, rows, tuple(table.shape), flush=True)
+                out = torch.full((rows, 4 * H, d), 77.0, dtype=q.dtype, device=DEV)
+                tq4.kv8_paged_prefill(q[:rows].to(DEV), kc, vc, sc, table,
+                                      dev(np.array(lens, np.int32)), dev(cu), 120, out=out)
+                torch.cuda.synchronize()
+                assert (out[torch.from_numpy(~done[:rows]).to(DEV)] == 77.0).all()
+                at = torch.from_numpy(done[:rows]).to(DEV)
+                ref.check(out[at], want[:rows][done[:rows]], off[:rows][done[:rows]], q.dtype)
+
+
+@pytest.mark.parametrize("S,d", [(1024, 64), (1024, 256), (80, 128), (16, 256), (512, 128)])
+def test_page_sizes(tq4, S, d):
+    """Pages of many strips and of odd counts of them, written and attended over."""
+    r = np.random.default_rng(S + d)
+    lens = [S + 17, 5, 2 * S]
+    kc, vc, sc = tq4.kv8_cache(9, 2, S, d)
+    order = r.permutation(9)
+    tables = np.full((3, 3), -1, np.int32)
+    slots, at = [], 0
+    for b, n in enumerate(lens):
+        for i in range(-(-n // S)):
+            tables[b, i] = order[at]
+            at += 1
+        slots += [tables[b, i // S] * S + i % S for i in range(n)]
+    k, v = queries(r, sum(lens), 2, d, "bf16"), queries(r, sum(lens), 2, d, "bf16", 5.0)
+    tq4.kv8_reshape_and_cache(k.to(DEV), v.to(DEV), kc, vc, sc, dev(np.array(slots, np.int32)))
+    raw = [x.view(torch.uint8).cpu().numpy() for x in (kc, vc)] + [sc.cpu().numpy()]
+    empty = [np.zeros_like(x) for x in raw]
+    want = ref.write(k.float().numpy(), v.float().numpy(), *empty, np.array(slots), "fp8")
+    assert all(np.array_equal(a, b) for a, b in zip(raw, want))
+    check_decode(tq4, queries(r, 3, 8, d, "bf16"), (*raw, tables), lens, "fp8")
+    check_prefill(tq4, queries(r, 70, 4, d, "bf16"), (*raw, tables), lens, [60, 1, 9], "fp8", True)
+
+
+def test_nothing_to_do(tq4):
+    """No sequences, no rows, no tokens: nothing is launched, nothing refused."""
+    kc, vc, sc = tq4.kv8_cache(3, 2, 16, 64)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=DEV)  # noqa: E731
+    rows = lambda n, h: torch.ones((n, h, 64), dtype=torch.bfloat16, device=DEV)  # noqa: E731
+    tq4.kv8_reshape_and_cache(rows(0, 2), rows(0, 2), kc, vc, sc, i32(0))
+    assert tq4.kv8_paged_decode(rows(0, 4), kc, vc, sc, i32(0, 2), i32(0)).shape == (0, 4, 64)
+    none = tq4.kv8_paged_prefill(rows(0, 4), kc, vc, sc, i32(2, 2), i32(2), i32(3), 5)
+    assert none.shape == (0, 4, 64)
+    out = rows(3, 4)
+    tq4.kv8_paged_prefill(rows(3, 4), kc, vc, sc, i32(2, 2), i32(2), i32(3), 0, out=out)
+    tq4.kv8_paged_prefill(rows(3, 4), kc, vc, sc, i32(0, 2), i32(0), i32(1), 3, out=out)
+    assert (out == 1).all() and (sc == 0).all()
+
+
 @pytest.mark.parametrize("code", ["fp8", "int8"])
 def test_prefill_scales_far_apart(tq4, code):
     r = np.random.default_rng(13)

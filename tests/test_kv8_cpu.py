@@ -66,6 +66,9 @@ def test_attention_refusals_and_sizes(lib):
     assert dec(Hq=9) == dec(Hq=34) == dec(Hq=0) == dec(M=0) == dec(el=3) == dec(qs=512) == -3
     assert dec(K=257) == -5
     assert dec(M=2 ** 28) == dec(P=2 ** 28) == -10
+    # the join's rows: workgroups of 1024 behind more than 32 parts
+    many = dict(B=2 ** 18 - 1, Hq=17, H=17, qs=17 * 128, M=8)
+    assert dec(K=33, **many) == -10 and dec(K=32, **many) == -6
     assert dec(q=None) == dec(out=None) == pre(cu=None) == -1
     assert dec(q=ODD) == dec(qs=1028) == -14
     need = lib.tq4_kv8_decode_workspace_bytes(2, 8, 2, 128, 16, 64, 4)
