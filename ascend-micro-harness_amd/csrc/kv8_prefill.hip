@@ -17,8 +17,8 @@
 // and tile j + 2 comes from memory.
 //
 // Arithmetic bounds it: 8192 causal rows of 32 heads of 128 (8 KV heads) 584 us, 940
-// TFLOP/s where a library product of f16 matrices reaches 1336; 64 channels 365 us,
-// 750; 256 925 us, 595 (its 32 rows fill a wave's registers: one wave a SIMD). Without
+// TFLOP/s where a library product of f16 matrices reaches 1336; 64 channels 370 us,
+// 740; 256 865 us, 635 (its 32 rows fill a wave's registers: one wave a SIMD). Without
 // the softmax and the widening the products took 426 us of 616 (before the ring of
 // operand blocks); each added about 100. Beyond the ring, issue order is not what
 // holds it: priorities for one of a SIMD's two waves, a wave half a tile behind the
@@ -303,8 +303,10 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
 
         // The tile's operand blocks in the order of their MFMA: the keys of both
         // blocks of tokens, then the values strip by strip. A ring of registers
-        // holds the next kRing of them, or each MFMA would wait for its LDS read.
-        constexpr int kRing = 4, kScores = 2 * KK;
+        // holds the next kRing of them, or each MFMA would wait for its LDS read (8192
+        // rows of 32 heads of 128: 616 us without, 597 with four, 594 with eight; 256
+        // channels leave registers for two: 865 us, 930 with four).
+        constexpr int kRing = D == 256 ? 2 : 4, kScores = 2 * KK;
         h8_t ring[kRing];
         auto operand = [&](int i) {
             const int to = i < kScores ? i * Tile<D>::kKeyBlock
