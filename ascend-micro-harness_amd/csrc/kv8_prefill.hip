@@ -16,7 +16,7 @@
 // Two LDS buffers: tile j is computed while tile j + 1 is widened into the other
 // and tile j + 2 comes from memory.
 //
-// Arithmetic bounds it: 8192 causal rows of 32 heads of 128 (8 KV heads) 584 us, 940
+// Arithmetic bounds it: 8192 causal rows of 32 heads of 128 (8 KV heads) 590 us, 930
 // TFLOP/s where a library product of f16 matrices reaches 1336; 64 channels 370 us,
 // 740; 256 865 us, 635 (its 32 rows fill a wave's registers: one wave a SIMD). Without
 // the softmax and the widening the products took 426 us of 616 (before the ring of
