@@ -68,11 +68,14 @@ struct Stage {
     static constexpr int kThreads = 64 * W, kPieces = 4 * D;
     static constexpr int N = (kPieces + kThreads - 1) / kThreads;
     u4_t k[N], v[N];
-    int live[N];    // live tokens of the pieces' strips
-    int32_t e[N];   // the next fetch's block-table entries, -1: no page
-    int32_t es;     // the same of strip threadIdx.x % 4, its scales and live tokens
-    float ks, vs;
+    int live[N];   // live tokens of the pieces' strips
+    int32_t e[N];  // the next fetch's block-table entries, as they come from memory
+    int32_t es;    // lanes 0 to 3 of the first wave: the same of strip `lane`, its
+    float ks, vs;  // scales and live tokens
     int own;
+    uint32_t zero;  // 0, in a vector register
+
+    __device__ __forceinline__ Stage() { asm("v_mov_b32 %0, 0" : "=v"(zero)); }
 
     // (a wave too many brings another's pieces, and does not store them)
     static __device__ __forceinline__ uint32_t piece(int r)
@@ -83,27 +86,38 @@ struct Stage {
     {
         return __builtin_amdgcn_readfirstlane(piece(r) / D);
     }
-    static __device__ __forceinline__ int live_of(int32_t e, uint32_t L, uint32_t strip)
+    static __device__ __forceinline__ bool first_wave()
+    {
+        return __builtin_amdgcn_readfirstlane(threadIdx.x / 64) == 0;
+    }
+    // (past the table lies past the context too)
+    static __device__ __forceinline__ int live_of(const Kv8AttnParams& p, int32_t e, uint32_t L,
+                                                  uint32_t strip)
     {
         const int left = (int)L - (int)(16 * strip);
-        return e < 0 || left < 0 ? 0 : left > 16 ? 16 : left;
+        return e < 0 || (uint32_t)e >= p.P || left < 0 ? 0 : left > 16 ? 16 : left;
+    }
+    static __device__ __forceinline__ uint32_t page_of(const Kv8AttnParams& p, int32_t e)
+    {
+        return e < 0 || (uint32_t)e >= p.P ? 0u : (uint32_t)e;
     }
 
-    __device__ __forceinline__ int32_t entry(const Kv8AttnParams& p, const int32_t* table,
-                                             Divisor per_page, uint32_t strip) const
+    static __device__ __forceinline__ uint32_t index(const Kv8AttnParams& p, Divisor per_page,
+                                                     uint32_t strip)
     {
         const uint32_t i = div_by(strip, per_page);
-        const int32_t e = table[i < p.M ? i : p.M - 1];
-        return i < p.M && e >= 0 && (uint32_t)e < p.P ? e : -1;
+        return i < p.M ? i : p.M - 1;
     }
+    // Nothing here looks at what it loads: that would wait for it, once a tile.
     __device__ __forceinline__ void entries(const Kv8AttnParams& p, const int32_t* table,
                                             Divisor per_page, uint32_t t0)
     {
-#pragma unroll
         // (a vector load, though one entry a wave: a scalar one is waited for together
         // with the wave's LDS reads)
-        for (int r = 0; r < N; ++r) e[r] = entry(p, table, per_page, t0 / 16 + piece(r) / D);
-        es = entry(p, table, per_page, t0 / 16 + (threadIdx.x & 3u));
+#pragma unroll
+        for (int r = 0; r < N; ++r)
+            e[r] = table[index(p, per_page, t0 / 16 + strip_of(r)) + zero];
+        if (first_wave()) es = table[index(p, per_page, t0 / 16 + (threadIdx.x & 3u))];
     }
     __device__ __forceinline__ void fetch(const Kv8AttnParams& p, Divisor per_page, uint32_t h,
                                           uint32_t L, uint32_t t0)
@@ -111,19 +125,20 @@ struct Stage {
 #pragma unroll
         for (int r = 0; r < N; ++r) {
             const uint32_t u = piece(r), strip = t0 / 16 + strip_of(r);
-            const int32_t page = __builtin_amdgcn_readfirstlane(e[r]);
+            const int32_t entry = __builtin_amdgcn_readfirstlane(e[r]);
             const uint32_t in = strip - div_by(strip, per_page) * (p.S / 16);
-            const uint64_t at =
-                (((uint64_t)(uint32_t)(page < 0 ? 0 : page) * p.Hkv + h) * p.S + in * 16) * D;
+            const uint64_t at = (((uint64_t)page_of(p, entry) * p.Hkv + h) * p.S + in * 16) * D;
             // a strip's keys and values are 16 * D consecutive bytes, its pieces in order
             k[r] = *(const u4_t*)(p.key_cache + at + 16 * (u % D));
             v[r] = *(const u4_t*)(p.value_cache + at + 16 * (u % D));
-            live[r] = live_of(page, L, strip);
+            live[r] = live_of(p, entry, L, strip);
         }
-        const uint64_t row = (uint64_t)(uint32_t)(es < 0 ? 0 : es) * p.Hkv + h;
-        ks = p.scales[row];
-        vs = p.scales[(uint64_t)p.P * p.Hkv + row];
-        own = live_of(es, L, t0 / 16 + (threadIdx.x & 3u));
+        if (first_wave()) {
+            const uint64_t row = (uint64_t)page_of(p, es) * p.Hkv + h;
+            ks = p.scales[row];
+            vs = p.scales[(uint64_t)p.P * p.Hkv + row];
+            own = live_of(p, es, L, t0 / 16 + (threadIdx.x & 3u));
+        }
     }
     __device__ __forceinline__ void store(char* tile, StripInfo* info) const
     {
