@@ -201,8 +201,8 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
     constexpr int KK = D / 16, CB = D / 32;
     __shared__ __align__(16) char lds[2 * Tile<D>::kBytes];
     __shared__ StripInfo info[2][kStrips];
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
-    const uint32_t n = lane & 31u, half = lane >> 5;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t lane = threadIdx.x & 63u, n = lane & 31u, half = lane >> 5;
 
     // the heads of a tile lie next to each other in the grid (one an XCD, where
     // there are eight), then the parts of its tokens; a sequence's last tiles, the
@@ -385,12 +385,12 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
 #pragma unroll
         for (int x = 0; x < kStrips; ++x) {
             const float off = st[x].lv - m;
-            float sum = 0.0f;
+            float sum;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float e = __builtin_amdgcn_exp2f(
                     __builtin_fmaf(s[x / 2][8 * (x & 1) + i], fac[x], off));
-                sum += e;
+                sum = i ? sum + e : e;
                 pr[x][i] = (_Float16)e;
             }
             l += sum * st[x].rvs;
