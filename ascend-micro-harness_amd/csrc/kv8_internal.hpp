@@ -52,12 +52,13 @@ struct Kv8AttnParams {
     int causal;
     float scale;
 };
-// Waves of a prefill workgroup, 32 rows each (kv8_prefill.hip), for so many rows of
-// a (sequence, kv head) over tables of `cap` tokens, and the workgroups that the CUs
+// Waves of a prefill workgroup, 32 rows each (kv8_prefill.hip), for so many rows of a
+// (sequence, kv head) over tables of `cap` tokens, and the workgroups that the CUs
 // hold at once. Eight waves widen a tile for twice the rows (8192 rows x 32 heads of
-// 128: 619 us against 651), four are the more balanced where there are few tiles
-// (2048 rows: 72 us against 81; 1000: 37, 42); heads of 64 run better as three workgroups of four a CU (418 against 376 us), and
-// 256 channels fill a wave's registers and a CU's LDS with four.
+// 128: 619 us against 651), four are the more balanced where there are few tiles (2048
+// rows: 72 us against 81; 1000: 37, 42); heads of 64 run better as three workgroups of
+// four a CU (376 us against 418 with eight waves), and 256 channels fill a wave's
+// registers and a CU's LDS with four.
 inline uint32_t kv8_prefill_waves(uint32_t d, uint64_t rows, uint64_t cap)
 {
     return d == 128 && rows > 128 && cap > 2048 ? 8 : 4;

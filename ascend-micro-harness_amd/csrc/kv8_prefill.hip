@@ -19,13 +19,13 @@
 // Arithmetic bounds it: 8192 causal rows of 32 heads of 128 (8 KV heads) 557 us, 987
 // TFLOP/s where a library product of f16 matrices reaches 1336; 64 channels 355 us,
 // 775; 256 800 us, 690 (its 32 rows fill a wave's registers: one wave a SIMD). (Cards
-// and their clocks differ by 6%.) Without the softmax and the widening the products
-// took 426 us of 616, before the ring of operand blocks and before nothing waited for
-// a table entry; each added about 100. Beyond that, issue order is not what holds it:
-// priorities for one of a SIMD's two waves, a wave half a tile behind the other, and a
-// tile's softmax beside the next one's scores in one wave all took as long or longer.
-// 64 rows a wave halve the LDS reads, but their sums move through the accumulation
-// registers, which cost more.
+// and their clocks differ by 6%.) An earlier form, of 616 us, took 426 without the
+// softmax and the widening, which added about 100 each; a ring of operand blocks and
+// table entries that nothing waits for made up the difference. Issue order otherwise
+// is not what holds it: priorities for one of a SIMD's two waves, a wave half a tile
+// behind the other, and a tile's softmax beside the next one's scores in one wave all
+// took as long or longer. 64 rows a wave halve the LDS reads, but their sums move
+// through the accumulation registers, which cost more.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
