@@ -16,7 +16,6 @@ attention).
 """
 from __future__ import annotations
 
-import functools
 import importlib
 import math
 import random
@@ -32,7 +31,6 @@ TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 LEAST_SCALE = 2.0 ** -100
 
 
-@functools.lru_cache(None)
 def _package():
     return importlib.import_module("ascend-micro-harness_amd")
 
