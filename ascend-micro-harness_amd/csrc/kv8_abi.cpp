@@ -93,14 +93,15 @@ uint32_t record_rows(uint64_t max_q, uint64_t group)
     return (uint32_t)(max_q * group < tq4::kKv8Rows ? max_q * group : tq4::kKv8Rows);
 }
 
-// Records of a call: (floats of a row's sums, and two statistics) a row and slot.
+// Records of a call: (floats of a row's sums, and its statistics) a row and slot.
 uint64_t record_slots(const Cut& c, uint64_t items)
 {
     return c.K == 1 ? 0 : c.K ? mul(items, c.K) : 2ull * c.groups;
 }
 size_t record_bytes(const Cut& c, uint64_t items, uint32_t rec_rows, uint32_t d)
 {
-    const uint64_t b = mul(mul(record_slots(c, items), rec_rows), (uint64_t)d + 2, sizeof(float));
+    const uint64_t b =
+        mul(mul(record_slots(c, items), rec_rows), (uint64_t)d + tq4::kKv8Stats, sizeof(float));
     return b > (uint64_t)SIZE_MAX - 16 ? SIZE_MAX : (size_t)((b + 15) & ~15ull);
 }
 
@@ -195,7 +196,7 @@ tq4::Kv8AttnParams make(const void* q, const void* kc, const void* vc, const flo
     const uint64_t items = (uint64_t)num_seqs * num_kv_heads *
                            tiles_of(max_q, num_heads / num_kv_heads);
     if (const uint64_t slots = record_slots(cut, items))
-        p.ml = p.acc + slots * p.rec_rows * head_size;
+        p.stats = p.acc + slots * p.rec_rows * head_size;
     p.out = out;
     p.q_stride = q_stride;
     p.rows = rows;
@@ -406,7 +407,7 @@ int tq4_kv8_paged_prefill(void* stream, int element_type, int code_type, const v
             return TQ4_ERR_RANGE;
         if (!room) return TQ4_ERR_WORKSPACE;
         tq4::Kv8AttnParams p = args(Cut{k, 0, 0});
-        p.ml = p.acc + (uint64_t)num_rows * num_heads * k * head_size;
+        p.stats = p.acc + (uint64_t)num_rows * num_heads * k * head_size;
         return launched(tq4::launch_kv8_prefill((hipStream_t)stream, element_type,
                                                 code_type == TQ4_KV8_INT8, p));
     }

@@ -6,12 +6,13 @@
 // a time:
 //   S = K Q^T     MFMA 16x16x32 f16, tokens x rows. Codes are exact in f16 and a
 //                 row of q is shifted by a power of two into f16's range.
-//   s' = S * (k scale * q factor) + log2(v scale)      log2 units
-//   P = 2^(s' - m), in f16 with the v scale inside it, so the row's largest
-//       product is 2^6 whatever the scales' spread; m moves when a row passes
-//       2^14 (lazily), and the sums with it
-//   O^T += V^T P^T   on V's codes;  l += P / v scale
-//   out = O / l
+//   s' = S * (k scale * q factor)                      log2 units
+//   P = 2^(s' + log2(v scale) - m), in f16 with the v scale inside it, so the row's
+//       largest product is 2^6 whatever the scales' spread; m moves when a row
+//       passes 2^14 (lazily), and the sums with it
+//   O^T += V^T P^T   on V's codes;  l += 2^(s' - s), as P times a strip's factor, where
+//       s moves like m (References): weights whose products round to 0 count in l
+//   out = O 2^m / (l 2^s)
 // Tile j of S holds tokens 4j .. 4j + 3 of each of the four strips, so a lane's
 // 16 scores are the 16 tokens of one strip (one scale each) for one row: they are
 // the P^T operand as they lie, and the V^T operand is a channel's 16 consecutive
@@ -206,7 +207,8 @@ struct Lane {
 template <int D>
 struct Sums {
     f4_t o[D / 16];
-    float m, l;
+    References ref;
+    float l;
 };
 
 // The units of a wave's part of an item.
@@ -217,7 +219,8 @@ __device__ __forceinline__ void attend_units(const Kv8AttnParams& p, const Lane<
     const uint32_t step = kWaves * kUnit, g = at.walk.g;
     const int32_t limit = at.limit;
     f4_t (&o)[D / 16] = sums.o;
-    float &m = sums.m, &l = sums.l;
+    References& ref = sums.ref;
+    float& l = sums.l;
     KeyBytes<D> k;
     ValueBytes<D> v;
     Entries e = at.walk.entries(at.first);
@@ -267,8 +270,7 @@ __device__ __forceinline__ void attend_units(const Kv8AttnParams& p, const Lane<
                     widen8<INT8>(k.x[j][i][2], k.x[j][i][3]), q[2 * i + 1], s[j], 0, 0, 0);
             }
         }
-        const float vs = held_scale(now.vs);
-        const float fac = held_scale(now.ks) * qf, lv = __builtin_amdgcn_logf(vs);
+        const float fac = held_scale(now.ks) * qf, lv = __builtin_amdgcn_logf(held_scale(now.vs));
         const int live = now.live;
         __builtin_amdgcn_sched_barrier(0);
         next_keys();
@@ -280,7 +282,7 @@ __device__ __forceinline__ void attend_units(const Kv8AttnParams& p, const Lane<
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[j][i] = __builtin_fmaf(s[j][i], fac, lv);
+            for (int i = 0; i < 4; ++i) s[j][i] *= fac;
         if (__any(sees < 16)) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -292,27 +294,29 @@ __device__ __forceinline__ void attend_units(const Kv8AttnParams& p, const Lane<
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) most = fmaxf(most, s[j][i]);
-        if (__any(most > m + 14.0f)) {
+        if (__any(ref.passed(most + lv, most))) {
+            float product = most + lv;
+            product = fmaxf(product, xor_lanes(product, 16));
+            product = fmaxf(product, xor_lanes(product, 32));
             most = fmaxf(most, xor_lanes(most, 16));
             most = fmaxf(most, xor_lanes(most, 32));
-            const float to = fmaxf(m, most - 6.0f);
-            const float r = __builtin_amdgcn_exp2f(m - to);
-            m = to;
-            l *= r;
+            const References r = ref.moved_to(product, most);
+            l *= r.s;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) o[i] *= r;
+            for (int i = 0; i < D / 16; ++i) o[i] *= r.m;
         }
+        const float off = ref.exponent(lv);
         h8_t pr[2];
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float x = __builtin_amdgcn_exp2f(s[j][i] - m);
+                const float x = __builtin_amdgcn_exp2f(s[j][i] + off);
                 sum += x;
                 pr[j / 2][4 * (j & 1) + i] = (_Float16)x;
             }
-        l += sum * __builtin_amdgcn_rcpf(vs);
+        l += sum * ref.share(off);
         if (__any(live < 16)) {
             // a dead token's bytes may be a NaN: 0 times it is not 0
 #pragma unroll
@@ -351,14 +355,15 @@ __device__ __forceinline__ void attend_units(const Kv8AttnParams& p, const Lane<
 template <int D, int BF16, int INT8>
 __device__ __forceinline__ void merge_waves(const Kv8AttnParams& p, const Part& x,
                                             const Sums<D>& sums, float (*part)[kRows][D + 4],
-                                            float (*stat)[kRows][2])
+                                            float (*stat)[kRows][3])
 {
     const uint32_t wave = threadIdx.x >> 6, c = threadIdx.x & 15u, g = (threadIdx.x & 63u) >> 4;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) *(f4_t*)&part[wave][c][16 * i + 4 * g] = sums.o[i];
     if (g == 0) {
-        stat[wave][c][0] = sums.m;
-        stat[wave][c][1] = sums.l;
+        stat[wave][c][0] = sums.ref.m;
+        stat[wave][c][1] = sums.ref.s;
+        stat[wave][c][2] = sums.l;
     }
     __syncthreads();
     const uint32_t left = x.seq.rows * p.G - x.rt * kRows;
@@ -367,29 +372,26 @@ __device__ __forceinline__ void merge_waves(const Kv8AttnParams& p, const Part& 
         const uint32_t r = k / (D / 4), ch = (k % (D / 4)) * 4;
         const uint32_t fr = x.rt * kRows + r, row = x.seq.row0 + fr / p.G;
         if (row >= p.rows) break;
-        float mm = stat[0][r][0];
+        References to{stat[0][r][0], stat[0][r][1]};
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, stat[w][r][0]);
+        for (int w = 1; w < kWaves; ++w)
+            to = {fmaxf(to.m, stat[w][r][0]), fmaxf(to.s, stat[w][r][1])};
         f4_t a = {0, 0, 0, 0};
         float ll = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            const float s = __builtin_amdgcn_exp2f(stat[w][r][0] - mm);
-            ll += s * stat[w][r][1];
-            a += s * *(const f4_t*)&part[w][r][ch];
+            ll += __builtin_amdgcn_exp2f(stat[w][r][1] - to.s) * stat[w][r][2];
+            a += __builtin_amdgcn_exp2f(stat[w][r][0] - to.m) * *(const f4_t*)&part[w][r][ch];
         }
         if (x.slot < 0) {
-            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+            const Quotient y(to, ll);
             const uint64_t at = (uint64_t)row * p.Hq + x.h * p.G + fr % p.G;
             *(u2_t*)((uint16_t*)p.out + at * D + ch) =
-                u2_t{narrow2<BF16>(a[0] * inv, a[1] * inv), narrow2<BF16>(a[2] * inv, a[3] * inv)};
+                u2_t{narrow2<BF16>(y(a[0]), y(a[1])), narrow2<BF16>(y(a[2]), y(a[3]))};
         } else {
             const uint64_t rec = (uint64_t)x.slot * p.rec_rows + r;
             *(f4_t*)(p.acc + rec * D + ch) = a;
-            if (ch == 0) {
-                p.ml[2 * rec] = mm;
-                p.ml[2 * rec + 1] = ll;
-            }
+            if (ch == 0) *(f4_t*)(p.stats + kKv8Stats * rec) = f4_t{to.m, to.s, ll, 0.0f};
         }
     }
 }
@@ -399,7 +401,7 @@ __global__ __launch_bounds__(kThreads, kKv8GroupsPerCu(D)) void kv8_decode(Kv8At
                                                                            Divisor per_page)
 {
     __shared__ float part[kWaves][kRows][D + 4];
-    __shared__ float stat[kWaves][kRows][2];
+    __shared__ float stat[kWaves][kRows][3];
     const uint32_t lane = threadIdx.x & 63u;
     Part x;
     uint32_t left = 0;  // units of the workgroup behind this part
@@ -486,7 +488,7 @@ __global__ __launch_bounds__(kThreads, kKv8GroupsPerCu(D)) void kv8_decode(Kv8At
         Sums<D> sums;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) sums.o[i] = f4_t{0, 0, 0, 0};
-        sums.m = kNone;
+        sums.ref = References::none();
         sums.l = 0.0f;
         const Lane<D> at(p, per_page, x);
         if (at.units) attend_units<D, BF16, INT8>(p, at, sums);

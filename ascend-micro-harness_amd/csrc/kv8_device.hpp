@@ -17,7 +17,69 @@ typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNone = -3.0e38f;  // the running maximum before any token
+constexpr float kNone = -3.0e38f;  // a running maximum before any token
+
+// What a row's sums are held against, in log2 units and whole numbers: the products
+// (weight times value scale) against 2^m, the weights against 2^s. They are two, as
+// the value scales of a context may lie far apart: a page of zeros has 2^-100.
+struct References {
+    float m, s;
+
+    __device__ __forceinline__ static References none() { return {kNone, kNone}; }
+    // Both moved up to bring the largest product and weight to 2^6 .. 2^7, which leaves
+    // the sums room until one passes 2^14; what each sum is multiplied by.
+    __device__ __forceinline__ References moved_to(float product, float weight)
+    {
+        const References was = *this;
+        m = fmaxf(m, floorf(product - 6.0f));
+        s = fmaxf(s, floorf(weight - 6.0f));
+        return {__builtin_amdgcn_exp2f(was.m - m), __builtin_amdgcn_exp2f(was.s - s)};
+    }
+    __device__ __forceinline__ bool passed(float product, float weight) const
+    {
+        return product > m + 14.0f || weight > s + 14.0f;
+    }
+    // The product of score x in a strip of value scale 2^lv is 2^(x + exponent(lv)), its
+    // weight share(exponent) times that. A strip all of whose products lie below 2^-26,
+    // which FP16 rounds to 0, has them at 2^-40 times its weights instead: these count
+    // in their sum whatever its scale is, down to 2^-86 of the row's largest.
+    __device__ __forceinline__ float exponent(float lv) const { return fmaxf(lv - m, -40.0f - s); }
+    __device__ __forceinline__ float share(float exponent) const
+    {
+        return __builtin_amdgcn_exp2f(-(exponent + s));
+    }
+    // The same with less of it a tile, for strips whose lv and 2^8 / scale are at hand:
+    // exponent lv - m and share rvs * gap(), once `hold` has seen the strips of a tile
+    // for which `passes_or_holds`, lv the least of theirs (so a weight maybe passes). The
+    // gap is at most 2^123 for scales up to 2^122. (8192 rows of 32 heads of 128: 573 us
+    // with the above, 564 so; the decode spills with it.)
+    __device__ __forceinline__ bool passes_or_holds(float product, float lv) const
+    {
+        return product > fminf(m, s + lv) + 14.0f || s + lv < m - 40.0f;
+    }
+    __device__ __forceinline__ void hold(float& lv, float& rvs) const
+    {
+        lv = fmaxf(lv, m - s - 40.0f);
+        rvs = fminf(rvs, __builtin_amdgcn_exp2f(s - m + 48.0f));
+    }
+    __device__ __forceinline__ float gap() const { return __builtin_amdgcn_exp2f(m - s - 8.0f); }
+};
+
+// The sums of a row, o and l, as its output o 2^m / (l 2^s); 0 where it saw nothing.
+struct Quotient {
+    float inv;
+    int up;
+
+    __device__ __forceinline__ Quotient(References r, float l)
+        : inv(l == 0.0f ? 0.0f : 1.0f / l),
+          up((int)fminf(fmaxf(r.m - r.s, -400.0f), 400.0f))
+    {
+    }
+    __device__ __forceinline__ float operator()(float o) const
+    {
+        return __builtin_amdgcn_ldexpf(o * inv, up);
+    }
+};
 
 // Four codes of a word as f16 (exact for both types).
 template <int INT8>
@@ -173,7 +235,7 @@ __device__ __forceinline__ uint32_t sequence_of(const Kv8AttnParams& p, uint32_t
     return lo;
 }
 
-// The records of output row `at`, weights 2^(m_k - max m), to the output. TEAM
+// The records of output row `at`, each moved to the largest references, to the output. TEAM
 // waves take them in turn and merge in `part` (TEAM rows; one wave: not used).
 // record(k): the index of record k < bound; count(): how many of them were written,
 // fewer than 2 where the row is none of the join's. The first loads do not wait for
@@ -195,26 +257,32 @@ __device__ __forceinline__ void join_records(const Kv8AttnParams& p, uint64_t at
         }
     };
     auto stat = [&](uint32_t k) {
-        return k < bound ? *(const float2*)(p.ml + 2 * record(k)) : float2{kNone, 0.0f};
+        return k < bound ? *(const f4_t*)(p.stats + kKv8Stats * record(k))
+                         : f4_t{kNone, kNone, 0.0f, 0.0f};
     };
-    float2 st = stat(lane);
+    f4_t st = stat(lane);
     load(0, mine, bound - 1);
     const uint32_t K = count();
     if (K < 2) return;
-    float m = kNone, a[C] = {}, l = 0.0f;
+    References ref = References::none();
+    float a[C] = {}, l = 0.0f;
     for (uint32_t k0 = 0; k0 < K; k0 += 64) {
         if (k0) {
             st = stat(k0 + lane);
             load(k0, mine, K - 1);
         }
         const bool held = k0 + lane < K;
-        float to = held ? fmaxf(m, st.x) : m;
+        const References was = ref;
+        if (held) ref = {fmaxf(ref.m, st[0]), fmaxf(ref.s, st[1])};
 #pragma unroll
-        for (int i = 1; i < 64; i <<= 1) to = fmaxf(to, xor_lanes(to, i));
-        const float r = __builtin_amdgcn_exp2f(m - to);
-        m = to;
-        const float w = held ? __builtin_amdgcn_exp2f(st.x - m) : 0.0f;  // of record k0 + lane
-        l = held ? l * r + w * st.y : l * r;
+        for (int i = 1; i < 64; i <<= 1) {
+            ref.m = fmaxf(ref.m, xor_lanes(ref.m, i));
+            ref.s = fmaxf(ref.s, xor_lanes(ref.s, i));
+        }
+        const float r = __builtin_amdgcn_exp2f(was.m - ref.m);
+        const float w = held ? __builtin_amdgcn_exp2f(st[0] - ref.m) : 0.0f;  // of record k0 + lane
+        l *= __builtin_amdgcn_exp2f(was.s - ref.s);
+        l = held ? l + __builtin_amdgcn_exp2f(st[1] - ref.s) * st[2] : l;
 #pragma unroll
         for (int i = 0; i < C; ++i) a[i] *= r;
         const uint32_t n = K - k0 < 64 ? K - k0 : 64u;
@@ -242,14 +310,13 @@ __device__ __forceinline__ void join_records(const Kv8AttnParams& p, uint64_t at
 #pragma unroll
             for (int i = 0; i < C; ++i) a[i] += part[t][lane * C + i];
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const Quotient y(ref, l);
     uint16_t* out = (uint16_t*)p.out + at * D + lane * C;
     if constexpr (C == 1) {
-        *out = (uint16_t)narrow2<BF16>(a[0] * inv, 0.0f);
+        *out = (uint16_t)narrow2<BF16>(y(a[0]), 0.0f);
     } else {
 #pragma unroll
-        for (int i = 0; i < C; i += 2)
-            *(uint32_t*)(out + i) = narrow2<BF16>(a[i] * inv, a[i + 1] * inv);
+        for (int i = 0; i < C; i += 2) *(uint32_t*)(out + i) = narrow2<BF16>(y(a[i]), y(a[i + 1]));
     }
 }
 

@@ -33,6 +33,7 @@ hipError_t launch_kv8_writer(hipStream_t stream, int bf16, int int8, const Kv8Wr
 
 // Attention; cu NULL: one row a sequence.
 constexpr uint32_t kKv8Unit = 64, kKv8Rows = 16;  // tokens of a step, rows of a tile
+constexpr uint32_t kKv8Stats = 4;  // of a record's row: its References, its sum, one unused
 // Workgroups of the decode that a CU holds at once, by registers.
 constexpr int kKv8GroupsPerCu(int d) { return d == 256 ? 1 : d == 128 ? 2 : 4; }
 
@@ -41,7 +42,7 @@ struct Kv8AttnParams {
     const uint8_t *key_cache, *value_cache;
     const float* scales;
     const int32_t *tables, *context_lens, *cu;
-    float *acc, *ml;  // records: [slot][rec_rows][D] and [slot][rec_rows][2]
+    float *acc, *stats;  // records: [slot][rec_rows][D] and [slot][rec_rows][kKv8Stats]
     void* out;
     uint64_t q_stride;
     uint32_t rows, B, Hq, Hkv, G, D, S, P, M;

@@ -5,9 +5,9 @@
 // the GQA group's heads, so the group shares each key. A wave has 32 of them and
 // walks the tokens 64 at a time with its workgroup:
 //   S = K Q^T       MFMA 32x32x16 f16, 32 tokens x 32 rows
-//   s' = S * (k scale * q factor) + log2(v scale)
-//   P = 2^(s' - m)  in f16, the v scale inside it (kv8_decode.hip)
-//   O^T += V^T P^T, l += P / v scale, out = O / l
+//   s' = S * (k scale * q factor)
+//   P = 2^(s' + log2(v scale) - m)  in f16, the v scale inside it (kv8_decode.hip)
+//   O^T += V^T P^T, l += 2^(s' - s), out = O 2^m / (l 2^s)
 // The tile's codes are widened to f16 once, on their way into LDS, in the order in
 // which the matrix operands are read (a lane's 16 bytes next to its neighbour's).
 // Tokens are permuted inside a block of 32 so that a lane's scores are, as they
@@ -56,7 +56,7 @@ struct Tile {
 };
 
 struct StripInfo {
-    float ks, lv, rvs;  // key scale, log2 and reciprocal of the value scale
+    float ks, lv, rvs;  // key scale, log2 of the value scale, 2^8 over it
     int live;           // its live tokens
 };
 
@@ -165,11 +165,11 @@ struct Stage {
             }
         }
         if (threadIdx.x < kStrips) {
-            const float s = held_scale(vs);
             StripInfo i;
             i.ks = held_scale(ks);
+            const float s = held_scale(vs);
             i.lv = __builtin_amdgcn_logf(s);
-            i.rvs = __builtin_amdgcn_rcpf(s);
+            i.rvs = 0x1.0p+8f * __builtin_amdgcn_rcpf(s);
             i.live = own;
             info[threadIdx.x] = i;
         }
@@ -244,7 +244,8 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
         limit = x < 0 ? 0 : (int32_t)x;
     }
     h8_t q[KK];
-    float qf, m = kNone, l = 0.0f;
+    float qf, l = 0.0f, gap = 0.0f;
+    References ref = References::none();
     f16_t o[CB];
     {
         uint32_t row = seq.row0 + fr / p.G;
@@ -363,29 +364,39 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
                 }
             }
         }
-        float fac[kStrips], most = -__builtin_inff();
+        float fac[kStrips], product = -__builtin_inff(), lv = st[0].lv;
+        auto largest = [&](int x) {
+            float y = s[x / 2][8 * (x & 1)];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) y = fmaxf(y, s[x / 2][8 * (x & 1) + i]);
+            return y;
+        };
 #pragma unroll
         for (int x = 0; x < kStrips; ++x) {
             // (not 0: a masked score is -inf)
             fac[x] = fmaxf(st[x].ks * qf, 1e-37f);
-            float y = s[x / 2][8 * (x & 1)];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) y = fmaxf(y, s[x / 2][8 * (x & 1) + i]);
-            most = fmaxf(most, __builtin_fmaf(y, fac[x], st[x].lv));
+            product = fmaxf(product, __builtin_fmaf(largest(x), fac[x], st[x].lv));
+            lv = fminf(lv, st[x].lv);
         }
-        if (__any(most > m + 14.0f)) {
-            most = fmaxf(most, xor_lanes(most, 32));
-            const float to = fmaxf(m, most - 6.0f);
-            const float r = __builtin_amdgcn_exp2f(m - to);
-            m = to;
-            l *= r;
+        if (__any(ref.passes_or_holds(product, lv))) {
+            float weight = largest(0) * fac[0];
 #pragma unroll
-            for (int c = 0; c < CB; ++c) o[c] *= r;
+            for (int x = 1; x < kStrips; ++x) weight = fmaxf(weight, largest(x) * fac[x]);
+            product = fmaxf(product, xor_lanes(product, 32));
+            weight = fmaxf(weight, xor_lanes(weight, 32));
+            const References r = ref.moved_to(product, weight);
+            l *= r.s;
+#pragma unroll
+            for (int c = 0; c < CB; ++c) o[c] *= r.m;
+            gap = ref.gap();
+#pragma unroll
+            for (int x = 0; x < kStrips; ++x) ref.hold(st[x].lv, st[x].rvs);
         }
         h8_t pr[kStrips];
+        float weights = 0.0f;
 #pragma unroll
         for (int x = 0; x < kStrips; ++x) {
-            const float off = st[x].lv - m;
+            const float off = st[x].lv - ref.m;
             float sum;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -394,8 +405,9 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
                 sum = i ? sum + e : e;
                 pr[x][i] = (_Float16)e;
             }
-            l += sum * st[x].rvs;
+            weights += sum * st[x].rvs;
         }
+        l += weights * gap;
 #pragma unroll
         for (int i = 0; i < kScores; ++i) {
             const int c = i % CB;
@@ -416,21 +428,18 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
             for (int x = 0; x < 4; ++x)
                 *(f4_t*)(p.acc + rec * D + 32 * c + 8 * x + 4 * half) =
                     f4_t{o[c][4 * x], o[c][4 * x + 1], o[c][4 * x + 2], o[c][4 * x + 3]};
-        if (half == 0) {
-            p.ml[2 * rec] = m;
-            p.ml[2 * rec + 1] = l;
-        }
+        if (half == 0) *(f4_t*)(p.stats + kKv8Stats * rec) = f4_t{ref.m, ref.s, l, 0.0f};
         return;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const Quotient y(ref, l);
     uint16_t* out = (uint16_t*)p.out + to * D + 4 * half;
 #pragma unroll
     for (int c = 0; c < CB; ++c)
 #pragma unroll
         for (int x = 0; x < 4; ++x)
             *(u2_t*)(out + 32 * c + 8 * x) =
-                u2_t{narrow2<BF16>(o[c][4 * x] * inv, o[c][4 * x + 1] * inv),
-                     narrow2<BF16>(o[c][4 * x + 2] * inv, o[c][4 * x + 3] * inv)};
+                u2_t{narrow2<BF16>(y(o[c][4 * x]), y(o[c][4 * x + 1])),
+                     narrow2<BF16>(y(o[c][4 * x + 2]), y(o[c][4 * x + 3]))};
 }
 
 // The parts of the rows, joined: D / 4 lanes a (row, head), as many workgroups as a
@@ -455,37 +464,35 @@ __global__ __launch_bounds__(256) void kv8_prefill_combine(Kv8AttnParams p)
         const Span span(p, s, f / group_rows(W) * group_rows(W), group_rows(W));
         if (span.each >= span.tiles) continue;  // one part: it went to the output
         const uint32_t parts = (span.tiles + span.each - 1) / span.each;
-        const float* ml = p.ml + 2 * at * p.K;
+        const float* stats = p.stats + kKv8Stats * at * p.K;
         // eight parts' loads at a time (past the last: its own again, left out)
-        float m = kNone, l = 0.0f;
+        References ref = References::none();
+        float l = 0.0f;
         f4_t a = {0, 0, 0, 0};
         for (uint32_t k0 = 0; k0 < parts; k0 += 8) {
-            float2 st[8];
+            f4_t st[8];
             f4_t x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const uint32_t k = k0 + j < parts ? k0 + j : parts - 1;
-                st[j] = *(const float2*)(ml + 2 * k);
+                st[j] = *(const f4_t*)(stats + kKv8Stats * k);
                 x[j] = *(const f4_t*)(p.acc + (at * p.K + k) * D + ch);
             }
-            float to = m;
+            const References was = ref;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) to = fmaxf(to, st[j].x);
-            const float r = __builtin_amdgcn_exp2f(m - to);
-            m = to;
-            l *= r;
-            a *= r;
+            for (int j = 0; j < 8; ++j) ref = {fmaxf(ref.m, st[j][0]), fmaxf(ref.s, st[j][1])};
+            l *= __builtin_amdgcn_exp2f(was.s - ref.s);
+            a *= __builtin_amdgcn_exp2f(was.m - ref.m);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 if (k0 + j >= parts) break;
-                const float w = __builtin_amdgcn_exp2f(st[j].x - m);
-                l += w * st[j].y;
-                a += w * x[j];
+                l += __builtin_amdgcn_exp2f(st[j][1] - ref.s) * st[j][2];
+                a += __builtin_amdgcn_exp2f(st[j][0] - ref.m) * x[j];
             }
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const Quotient y(ref, l);
         *(u2_t*)((uint16_t*)p.out + at * D + ch) =
-            u2_t{narrow2<BF16>(a[0] * inv, a[1] * inv), narrow2<BF16>(a[2] * inv, a[3] * inv)};
+            u2_t{narrow2<BF16>(y(a[0]), y(a[1])), narrow2<BF16>(y(a[2]), y(a[3]))};
     }
 }
 

@@ -1,0 +1,89 @@
+"""Value scales far apart in one context: a row's sum of weights must not depend
+on them. Against the definition in 64 bits, within kv8_reference's bound; its terms
+hold here, as a weight below 2^-86 of the row's largest, which an implementation may
+leave out of the sum, changes the sum of n weights by n 2^-86 at most, far below
+the 2^-24 a token that the bound has for sums."""
+import numpy as np
+import pytest
+import torch
+
+import kv8_reference as ref
+from test_gpu_kv8_attention import cache, check_decode, check_prefill, decode, queries
+
+pytestmark = pytest.mark.gpu
+
+CASES = [(64, 2, "fp8"), (128, 4, "int8"), (128, 1, "fp8"), (256, 8, "int8")]
+
+
+def zero_value_pages(c, tables, which):
+    """The pages `which` of every sequence hold values of 0, as the writer leaves
+    such pages: codes 0 at the least scale."""
+    for row in tables:
+        for i in which:
+            if i < len(row) and row[i] >= 0:
+                c[1][row[i]] = 0
+                c[2][1, row[i]] = ref.LEAST
+
+
+@pytest.mark.parametrize("top", [0, 34, 60, 110])
+@pytest.mark.parametrize("d,G,code", CASES)
+def test_zero_values_beside_large_ones(tq4, d, G, code, top):
+    """Equal scores, half of the tokens with values of 0: the others' mean, halved,
+    however large they are. The pages lie in one wave's tokens, in several waves',
+    in several parts."""
+    r = np.random.default_rng(d + top)
+    lens, S = [32, 160, 700], 16
+    c = cache(r, lens, 1, S, d, code, spread=1)
+    c[2][1] = 2.0 ** top
+    zero_value_pages(c, c[3], range(0, 44, 2))
+    q = torch.zeros((3, G, d), dtype=torch.bfloat16)
+    check_decode(tq4, q, c, lens, code)
+    for K in (1, 3, 11):
+        check_decode(tq4, q, c, lens, code, num_splits=K)
+    for rows in ([32, 160, 90], [1, 2, 3]):
+        q = torch.zeros((sum(rows), G, d), dtype=torch.bfloat16)
+        for causal in (True, False):
+            check_prefill(tq4, q, c, lens, rows, code, causal)
+
+
+@pytest.mark.parametrize("d,G,code", CASES)
+def test_value_scales_of_the_whole_range(tq4, d, G, code):
+    """Pages of every value scale from 2^-100 to 2^110 in one context, scores that
+    are equal, spread, and against the scales' order."""
+    r = np.random.default_rng(d)
+    lens, rows, S = [900, 300], [40, 150], 16
+    c = cache(r, lens, 1, S, d, code, spread=1)
+    exps = r.integers(-100, 111, c[2][1].shape)
+    c[2][1] = (2.0 ** exps).astype(np.float32)
+    for size in (0.0, 0.5, 8.0):
+        check_decode(tq4, queries(r, 2, G, d, "bf16", size), c, lens, code)
+        check_decode(tq4, queries(r, 2, G, d, "bf16", size), c, lens, code, num_splits=5)
+        q = queries(r, sum(rows), G, d, "bf16", size)
+        check_prefill(tq4, q, c, lens, rows, code, True)
+        check_prefill(tq4, q[:10], c, lens, [3, 7], code, True)
+    # rising along the context, then falling
+    for way in (1, -1):
+        for row in c[3]:
+            pages = row[row >= 0][::way]
+            c[2][1, pages, 0] = 2.0 ** np.round(np.linspace(-100, 110, len(pages)))
+        q = queries(r, sum(rows), G, d, "bf16")
+        check_prefill(tq4, q, c, lens, rows, code, True)
+        check_decode(tq4, q[:2], c, lens, code)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_many_tokens_of_zero_values(tq4, d):
+    """20000 tokens of zero values before 16 of large ones: the sum of their
+    weights stays a number."""
+    r = np.random.default_rng(d)
+    n, S = 20016, 16
+    c = cache(r, [n], 1, S, d, "fp8", spread=1)
+    c[2][1] = 2.0 ** 40
+    zero_value_pages(c, c[3], range(n // S - 1))
+    q = torch.zeros((1, 2, d), dtype=torch.bfloat16)
+    check_decode(tq4, q, c, [n], "fp8")
+    check_decode(tq4, q, c, [n], "fp8", num_splits=1)
+    check_prefill(tq4, torch.zeros((40, 2, d), dtype=torch.bfloat16), c, [n], [40], "fp8", False)
+    # and all of them zero
+    zero_value_pages(c, c[3], range(n // S))
+    assert (decode(tq4, q, c, [n], "fp8") == 0).all()
