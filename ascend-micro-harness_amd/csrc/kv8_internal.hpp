@@ -8,7 +8,7 @@
 namespace tq4 {
 
 constexpr float kKv8LeastScale = 0x1.0p-100f;
-constexpr float kKv8MostScale = 0x1.0p+120f;
+constexpr float kKv8MostScale = 0x1.0p+122f;  // 127 times it holds every BF16 value
 
 struct PlanParams {
     const int32_t *context_lens, *query_lens, *release;

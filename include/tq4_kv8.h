@@ -13,7 +13,8 @@
  *   code   TQ4_KV8_FP8: OCP FP8 e4m3 (largest 448); TQ4_KV8_INT8: signed,
  *          two's complement (largest 127); stored value = code * scale.
  * Scales are positive finite floats; the writer makes powers of two from 2^-100
- * on. The attention reads a scale outside [2^-100, 2^120] as the nearer end.
+ * on, up to 2^120 (FP8) and 2^122 (INT8), which hold the largest BF16 value. The
+ * attention reads a scale outside [2^-100, 2^122] as the nearer end.
  *
  * Supported shapes: head_size in {64, 128, 256}; block_size a multiple of 16,
  * at most 1024; GQA group num_heads / num_kv_heads in [1, 16]. Caches, activations and

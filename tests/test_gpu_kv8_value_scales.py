@@ -87,3 +87,49 @@ def test_many_tokens_of_zero_values(tq4, d):
     # and all of them zero
     zero_value_pages(c, c[3], range(n // S))
     assert (decode(tq4, q, c, [n], "fp8") == 0).all()
+
+
+@pytest.mark.parametrize("code", ["fp8", "int8"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_largest_magnitudes_come_back(tq4, d, code, monkeypatch):
+    """BF16 values up to the type's largest, written and attended over: what the
+    writer's scales stand for is what the attention reads. (Codes of FP8 reach 448,
+    of INT8 127, so their scales end at 2^120 and 2^122.)"""
+    monkeypatch.setattr(ref, "MOST", 2.0 ** 122)
+    S, H, top = 16, 1, 2.0 ** 120
+    # one token a sequence: its output is its value. Multiples of 4 * top and of
+    # 16 * top are codes of both types.
+    v = torch.zeros(4, H, d, dtype=torch.float64)
+    for row, most in enumerate((112.0, 128.0, 224.0, 255.0)):
+        v[row, 0, :8] = torch.tensor([most, -most, 64.0, -64.0, 128.0, 96.0, 0.0, -32.0]) * top
+    key = torch.ones(4, H, d)
+    kc, vc, sc = tq4.kv8_cache(4, H, S, d, ref.CODES[code])
+    slots = torch.arange(4, dtype=torch.int32, device="cuda") * S
+    tq4.kv8_reshape_and_cache(key.bfloat16().cuda(), v.bfloat16().cuda(), kc, vc, sc, slots)
+    # (row magnitudes of 128, 128, 224 and 255 times 2^120 over 448 or 127)
+    assert sc[1].log2().flatten().tolist() == ([119, 119, 119, 120] if code == "fp8" else
+                                               [121, 121, 121, 122])
+    q = torch.ones(4, 2, d, dtype=torch.bfloat16, device="cuda")
+    tables = torch.arange(4, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    lens = torch.ones(4, dtype=torch.int32, device="cuda")
+    far = torch.full((4, 60000), -1, dtype=torch.int32, device="cuda")
+    far[:, :1] = tables
+    cu = torch.arange(5, dtype=torch.int32, device="cuda")
+    q60 = torch.ones(4 * 60, 2, d, dtype=torch.bfloat16, device="cuda")
+    for out in (tq4.kv8_paged_decode(q, kc, vc, sc, tables, lens),
+                tq4.kv8_paged_decode(q, kc, vc, sc, far, lens),
+                tq4.kv8_paged_prefill(q, kc, vc, sc, tables, lens, cu, 1),
+                tq4.kv8_paged_prefill(q60, kc, vc, sc, far, lens, cu * 60, 60,
+                                      causal=False)[::60]):
+        got = out.double().cpu()
+        # (255 rounds to 256, which passes FP32: those two channels are infinite)
+        assert torch.equal(got[:3], v[:3].expand(3, 2, d))
+        assert torch.equal(got[3, :, 2:], v[3, :, 2:].expand(2, d - 2))
+    # the same magnitudes as keys, against queries as small
+    r = np.random.default_rng(d)
+    lens = [80, 33]
+    c = cache(r, lens, H, S, d, code)
+    c[2][0] = (2.0 ** r.integers(117, 121 if code == "fp8" else 123, c[2][0].shape))
+    q = (queries(r, 60, 2, d, "bf16").double() * 2.0 ** -124).bfloat16()
+    check_decode(tq4, q[:2], c, lens, code)
+    check_prefill(tq4, q, c, lens, [40, 20], code, True)
