@@ -152,7 +152,8 @@ uint32_t prefill_parts(uint32_t d, uint64_t num_rows, uint64_t seqs, uint64_t he
 bool cut_fits(const Cut& c, uint64_t seqs, uint64_t cap, uint64_t heads, uint64_t tiles,
               uint64_t rows)
 {
-    if (rows > (c.K > 32 ? kMaxGroups / 4 : kMaxGroups)) return false;
+    const uint32_t join = tq4::kv8_join_waves(c.K, c.groups, mul(seqs, heads, tiles));
+    if (rows > (join == 16 ? kMaxGroups / 4 : kMaxGroups)) return false;
     if (c.K) return mul(seqs, c.K) <= kMaxGroups && mul(heads, tiles) <= 65535u;
     return mul(mul(seqs, (cap + tq4::kKv8Unit - 1) / tq4::kKv8Unit), heads, tiles) <= 0xff000000ull;
 }

@@ -562,15 +562,12 @@ hipError_t launch_t(hipStream_t stream, const Kv8AttnParams& p)
                        div_magic(p.S / 16));
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.K == 1) return e;
-    // An item's records, were all alike: more waves a row where there are many (and
-    // then few rows). 128 records of 32 rows x 256: 13.6 us with one load at a time
-    // and four waves.
-    const uint64_t rows = (uint64_t)p.rows * p.Hq, items = (uint64_t)p.B * p.Hkv * tiles;
-    const uint64_t records = p.K ? p.K : p.groups / items;
-    if (records > 32)
+    const uint64_t rows = (uint64_t)p.rows * p.Hq;
+    const uint32_t waves = kv8_join_waves(p.K, p.groups, (uint64_t)p.B * p.Hkv * tiles);
+    if (waves == 16)
         hipLaunchKernelGGL((kv8_combine<D, BF16, 16>), dim3((uint32_t)rows), dim3(1024), 0, stream,
                            p, tiles);
-    else if (records > 8)
+    else if (waves == 4)
         hipLaunchKernelGGL((kv8_combine<D, BF16, 4>), dim3((uint32_t)rows), dim3(kThreads), 0,
                            stream, p, tiles);
     else

@@ -125,9 +125,10 @@ int tq4_kv8_reshape_and_cache(void* stream, int element_type, int code_type, con
  * results are the same every time. workspace: tq4_kv8_decode_workspace_bytes
  * bytes (0: none needed) for the same num_splits, 16-byte aligned, any contents;
  * calls that overlap in time need their own (TQ4_ERR_WORKSPACE).
- * num_seqs * splits < 2^24, rows * num_heads < 2^24 (2^22 with more than 32
- * splits), max_blocks_per_seq * block_size < 2^31, and in shares num_seqs *
- * num_kv_heads * (tokens of a table, in 64s) <= 0xff000000 (TQ4_ERR_RANGE). */
+ * num_seqs * splits < 2^24; rows * num_heads < 2^24, or 2^22 where the join has
+ * many records a row (more than 32 splits, or few sequences in shares);
+ * max_blocks_per_seq * block_size < 2^31; in shares num_seqs * num_kv_heads *
+ * (tokens of a table, in 64s) <= 0xff000000 (TQ4_ERR_RANGE). */
 #define TQ4_KV8_MAX_SPLITS 256u
 size_t tq4_kv8_decode_workspace_bytes(uint32_t num_seqs, uint32_t num_heads,
                                       uint32_t num_kv_heads, uint32_t head_size,
