@@ -93,6 +93,13 @@ def _one_device(what, first, tensors):
             raise ValueError(f"{what}: {name} is on {t.device}, {name0} on {t0.device}")
 
 
+def _sizes(what, **sizes):
+    """Sizes that the C ABI's 32 bits hold (ctypes would cut the others to them)."""
+    for name, n in sizes.items():
+        if not 0 <= n < 1 << 32:
+            raise ValueError(f"{what}: {name} must lie in [0, 2^32), got {n}")
+
+
 def _rows(what, name, t):
     """Activations [rows][heads][d], each row contiguous: the row stride in elements."""
     _need(what, name, t, tuple(_ELEMENTS), ndim=3)
@@ -144,6 +151,7 @@ def paged_plan(context_lens, query_lens, block_tables, free_pages, free_state, s
             cu_seqlens, granted, block_size, release, positions, new_context_lens, new_free_state,
             workspace, stream), what):
         return
+    _sizes(what, block_size=block_size)
     _need(what, "block_tables", block_tables, _INT, ndim=2)
     B, M = block_tables.shape
     _need(what, "context_lens", context_lens, _INT, numel=B)
@@ -241,6 +249,9 @@ def _room(nbytes, workspace, device):
 def kv8_decode_workspace_bytes(num_seqs, num_heads, num_kv_heads, head_size, block_size,
                                max_blocks_per_seq, num_splits=0):
     """Bytes of workspace that kv8_paged_decode needs (0: none); any contents."""
+    _sizes("kv8_decode_workspace_bytes", num_seqs=num_seqs, num_heads=num_heads,
+           num_kv_heads=num_kv_heads, head_size=head_size, block_size=block_size,
+           max_blocks_per_seq=max_blocks_per_seq, num_splits=num_splits)
     return int(_lib().tq4_kv8_decode_workspace_bytes(num_seqs, num_heads, num_kv_heads, head_size,
                                                      block_size, max_blocks_per_seq, num_splits))
 
@@ -280,6 +291,11 @@ def kv8_paged_decode(q, key_cache, value_cache, scale_cache, block_tables, conte
 def kv8_prefill_workspace_bytes(num_rows, num_seqs, num_heads, num_kv_heads, head_size,
                                 block_size, max_blocks_per_seq, max_query_len):
     """Bytes of workspace that kv8_paged_prefill needs (0: none); any contents."""
+    max_query_len = min(max_query_len, num_rows)
+    _sizes("kv8_prefill_workspace_bytes", num_rows=num_rows, num_seqs=num_seqs,
+           num_heads=num_heads, num_kv_heads=num_kv_heads, head_size=head_size,
+           block_size=block_size, max_blocks_per_seq=max_blocks_per_seq,
+           max_query_len=max_query_len)
     return int(_lib().tq4_kv8_prefill_workspace_bytes(num_rows, num_seqs, num_heads, num_kv_heads,
                                                       head_size, block_size, max_blocks_per_seq,
                                                       max_query_len))
@@ -307,6 +323,7 @@ def kv8_paged_prefill(q, key_cache, value_cache, scale_cache, block_tables, cont
     if max_query_len < 0:
         raise ValueError(f"{what}: max_query_len must not be negative, got {max_query_len}")
     T, Hq = q.shape[:2]
+    max_query_len = min(max_query_len, T)
     if scale is None:
         scale = 1.0 / math.sqrt(d)
     with _on(q.device, stream) as st:
