@@ -264,8 +264,9 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
         most = fmaxf(most, xor_lanes(most, 32));
         const float shift = row_shift(most);
         qf = (1.0f / shift) * (fabsf(p.scale) * kLog2e);
-        // a negative scale turns the row, so that larger products are larger scores
-        const float turned = p.scale < 0.0f ? -shift : shift;
+        // a negative scale turns the row, so that larger products are larger scores; one
+        // that is no number makes it such (fac is held at its least below)
+        const float turned = p.scale < 0.0f ? -shift : p.scale == p.scale ? shift : p.scale;
 #pragma unroll
         for (int i = 0; i < KK * 8; ++i) {
             const uint32_t w = raw[i / 8][(i / 2) & 3];
