@@ -180,15 +180,24 @@ struct Lane {
     Walk<D> walk;
     const uint16_t* q;  // the row's channels from the lane's on
     uint32_t first, units;
-    int32_t limit;
+    int32_t limit;     // tokens that the row sees
 
     __device__ __forceinline__ Lane(const Kv8AttnParams& p, Divisor per_page, const Part& x)
         : walk{&p, p.tables + (uint64_t)x.b * p.M, per_page, x.h, x.seq.tokens, threadIdx.x & 15u,
                (threadIdx.x & 63u) >> 4}
     {
-        const uint32_t wave = threadIdx.x >> 6;
-        first = (x.begin + wave) * kUnit;
-        units = x.begin + wave < x.end ? (x.end - x.begin - wave + kWaves - 1) / kWaves : 0u;
+        // tokens that no row of the tile sees are left out. Those that some rows see and
+        // others do not are fewer than kRows, in the last two units: a wave's last.
+        uint32_t end = x.end;
+        if (p.causal) {
+            const uint32_t last = x.rt * kRows + kRows - 1, rows = x.seq.rows * p.G;
+            walk.L = sees(x, (last < rows ? last : rows - 1) / p.G);
+            const uint32_t units = (walk.L + kUnit - 1) / kUnit;
+            end = end < units ? end : units;
+        }
+        const uint32_t wave = threadIdx.x >> 6, from = x.begin + wave;
+        first = from * kUnit;
+        units = from < end ? (end - from + kWaves - 1) / kWaves : 0u;
         // flat row f of the tile is token f / G, head f % G
         const uint32_t f = x.rt * kRows + walk.c, qi = f / p.G;
         const bool live = f < x.seq.rows * p.G && x.seq.row0 + qi < p.rows;
@@ -196,11 +205,13 @@ struct Lane {
             (uint64_t)(x.h * p.G + f % p.G) * D + 16u * walk.g;
         // tokens before `limit` (a lane without a row computes another's again,
         // unmasked, and drops it)
-        limit = (int32_t)x.seq.tokens;
-        if (p.causal && live) {
-            const int64_t t = (int64_t)x.seq.tokens - x.seq.all + qi + 1;
-            limit = t < 0 ? 0 : (int32_t)t;
-        }
+        limit = (int32_t)(p.causal && live ? sees(x, qi) : x.seq.tokens);
+    }
+    // tokens that row `qi` of a causal sequence sees
+    static __device__ __forceinline__ uint32_t sees(const Part& x, uint32_t qi)
+    {
+        const int64_t t = (int64_t)x.seq.tokens - x.seq.all + qi + 1;
+        return t < 0 ? 0u : (uint32_t)t;
     }
 };
 
@@ -211,10 +222,17 @@ struct Sums {
     float l;
 };
 
+// What the waves note of NaN codes (take_nan), each for itself.
+template <int D>
+struct Noted {
+    bool some[kWaves];
+    uint32_t first[kWaves][D];
+};
+
 // The units of a wave's part of an item.
 template <int D, int BF16, int INT8>
 __device__ __forceinline__ void attend_units(const Kv8AttnParams& p, const Lane<D>& at,
-                                             Sums<D>& sums)
+                                             Sums<D>& sums, Noted<D>& noted)
 {
     const uint32_t step = kWaves * kUnit, g = at.walk.g;
     const int32_t limit = at.limit;
@@ -257,7 +275,9 @@ __device__ __forceinline__ void attend_units(const Kv8AttnParams& p, const Lane<
     // the products: `next_keys` and `next_values` issue the next unit's loads
     // there, which then have the rest of this unit and the beginning of the next
     // to arrive.
-    auto take = [&](uint32_t t0, auto&& next_keys, auto&& next_values) {
+    // `last`: the wave's last unit, the only one that rows may see parts of.
+    auto take = [&](uint32_t t0, auto last, auto&& next_keys, auto&& next_values) {
+        constexpr bool kLast = decltype(last)::value;
         f4_t s[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -276,8 +296,11 @@ __device__ __forceinline__ void attend_units(const Kv8AttnParams& p, const Lane<
         next_keys();
         __builtin_amdgcn_sched_barrier(0);
         // the lane's tokens: strip g, token 4j + i; those it may see
-        const int ahead = limit - (int)(t0 + 16u * g);
-        const int sees = ahead < live ? (ahead < 0 ? 0 : ahead) : live;
+        int sees = live;
+        if constexpr (kLast) {
+            const int ahead = limit - (int)(t0 + 16u * g);
+            sees = ahead < live ? (ahead < 0 ? 0 : ahead) : live;
+        }
         float most = -__builtin_inff();
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -322,6 +345,22 @@ __device__ __forceinline__ void attend_units(const Kv8AttnParams& p, const Lane<
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) v.x[i] = live_bytes(v.x[i], live);
         }
+        if constexpr (kLast && !INT8) {
+            uint32_t nan = 0;
+            if (__any(sees < live)) {
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) nan |= nan_codes(v.x[i]);
+            }
+            if (p.causal && threadIdx.x % 64u == 0) noted.some[threadIdx.x / 64u] = false;
+            if (__any(nan)) {
+                uint32_t* first = noted.first[threadIdx.x / 64u];
+                for (uint32_t i = threadIdx.x % 64u; i < D; i += 64) first[i] = kNoToken;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+                    take_nan(v.x[i], t0 + 16u * g, &first[16 * i + at.walk.c]);
+                if (threadIdx.x % 64u == 0) noted.some[threadIdx.x / 64u] = true;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
             o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8<INT8>(v.x[i][0], v.x[i][1]),
@@ -337,7 +376,7 @@ __device__ __forceinline__ void attend_units(const Kv8AttnParams& p, const Lane<
     uint32_t t0 = at.first;
     for (uint32_t i = 1; i < at.units; ++i, t0 += step)
         take(
-            t0,
+            t0, Const<0>(),
             [&] {
                 next = at.walk.place(t0 + step, e);
                 e = at.walk.entries(t0 + 2 * step);
@@ -347,7 +386,7 @@ __device__ __forceinline__ void attend_units(const Kv8AttnParams& p, const Lane<
                 v.fetch(next.v);
                 now = next;
             });
-    take(t0, [] {}, [] {});
+    take(t0, Const<1>(), [] {}, [] {});
     l += xor_lanes(l, 16);
     l += xor_lanes(l, 32);
 }
@@ -355,7 +394,7 @@ __device__ __forceinline__ void attend_units(const Kv8AttnParams& p, const Lane<
 template <int D, int BF16, int INT8>
 __device__ __forceinline__ void merge_waves(const Kv8AttnParams& p, const Part& x,
                                             const Sums<D>& sums, float (*part)[kRows][D + 4],
-                                            float (*stat)[kRows][3])
+                                            float (*stat)[kRows][3], const Noted<D>& noted)
 {
     const uint32_t wave = threadIdx.x >> 6, c = threadIdx.x & 15u, g = (threadIdx.x & 63u) >> 4;
 #pragma unroll
@@ -383,6 +422,15 @@ __device__ __forceinline__ void merge_waves(const Kv8AttnParams& p, const Part& 
             ll += __builtin_amdgcn_exp2f(stat[w][r][1] - to.s) * stat[w][r][2];
             a += __builtin_amdgcn_exp2f(stat[w][r][0] - to.m) * *(const f4_t*)&part[w][r][ch];
         }
+        if (!INT8 && p.causal) {
+            for (int w = 0; w < kWaves; ++w) {
+                if (!noted.some[w]) continue;
+                const uint32_t sees = Lane<D>::sees(x, fr / p.G);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (noted.first[w][ch + i] < sees) a[i] = __builtin_nanf("");
+            }
+        }
         if (x.slot < 0) {
             const Quotient y(to, ll);
             const uint64_t at = (uint64_t)row * p.Hq + x.h * p.G + fr % p.G;
@@ -402,6 +450,7 @@ __global__ __launch_bounds__(kThreads, kKv8GroupsPerCu(D)) void kv8_decode(Kv8At
 {
     __shared__ float part[kWaves][kRows][D + 4];
     __shared__ float stat[kWaves][kRows][3];
+    __shared__ Noted<D> noted;
     const uint32_t lane = threadIdx.x & 63u;
     Part x;
     uint32_t left = 0;  // units of the workgroup behind this part
@@ -491,8 +540,9 @@ __global__ __launch_bounds__(kThreads, kKv8GroupsPerCu(D)) void kv8_decode(Kv8At
         sums.ref = References::none();
         sums.l = 0.0f;
         const Lane<D> at(p, per_page, x);
-        if (at.units) attend_units<D, BF16, INT8>(p, at, sums);
-        merge_waves<D, BF16, INT8>(p, x, sums, part, stat);
+        if (at.units) attend_units<D, BF16, INT8>(p, at, sums, noted);
+        else if (threadIdx.x % 64u == 0) noted.some[threadIdx.x / 64u] = false;
+        merge_waves<D, BF16, INT8>(p, x, sums, part, stat, noted);
         if (!following(x)) return;
         __syncthreads();  // the merge has read its sums
     }

@@ -16,6 +16,11 @@ typedef float f4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
 
+template <int N>
+struct Const {
+    static constexpr int value = N;
+};
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -3.0e38f;  // a running maximum before any token
 
@@ -190,6 +195,35 @@ __device__ __forceinline__ u4_t live_bytes(u4_t v, int live)
         v[i] &= m;
     }
     return v;
+}
+
+// NaN among the FP8 codes of values that some rows see and others do not: 0 times it
+// is not 0. Such codes are taken out; the first token of each channel that had one is
+// noted, and the sums of the rows that see it become NaN.
+constexpr uint32_t kNoToken = ~0u;
+
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w)  // their top bits
+{
+    return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+__device__ __forceinline__ uint32_t nan_codes(u4_t w)  // not 0 where there is one
+{
+    uint32_t some = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) some |= (w[i] & 0x7f7f7f7fu) + 0x01010101u;
+    return some & 0x80808080u;
+}
+// 16 tokens of a channel, the first of them `token`.
+__device__ __forceinline__ void take_nan(u4_t& w, uint32_t token, uint32_t* first)
+{
+    uint32_t at = kNoToken;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+        const uint32_t nan = (nan_codes(w[i]) >> 7) * 0xffu;
+        if (nan) at = token + 4 * i + __builtin_ctz(nan) / 8;
+        w[i] &= ~nan;
+    }
+    if (at != kNoToken) atomicMin(first, at);
 }
 
 // A sequence's rows and tokens, held in bounds.

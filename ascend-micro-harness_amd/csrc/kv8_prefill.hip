@@ -141,7 +141,10 @@ struct Stage {
             own = live_of(p, es, L, t0 / 16 + (threadIdx.x & 3u));
         }
     }
-    __device__ __forceinline__ void store(char* tile, StripInfo* info) const
+    // AGAIN: take_nan from the tile's values, whose first token is `token`.
+    template <int AGAIN>
+    __device__ __forceinline__ void store(char* tile, StripInfo* info, uint32_t* first_nan,
+                                          uint32_t token) const
     {
 #pragma unroll
         for (int r = 0; r < N; ++r) {
@@ -159,6 +162,7 @@ struct Stage {
                 u4_t w = v[r];
                 if (live[r] < 16) w = live_bytes(w, live[r]);
                 const uint32_t strip = u / D, c = u % D;
+                if constexpr (AGAIN) take_nan(w, token + 16 * strip, &first_nan[c]);
                 char* to = tile + Tile<D>::kKeys + (strip * (D / 32) + c / 32) * 1024 + (c % 32) * 16;
                 *(h8_t*)to = widen8<INT8>(w[0], w[1]);
                 *(h8_t*)(to + 512) = widen8<INT8>(w[2], w[3]);
@@ -202,6 +206,7 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
     constexpr int KK = D / 16, CB = D / 32;
     __shared__ __align__(16) char lds[2 * Tile<D>::kBytes];
     __shared__ StripInfo info[2][kStrips];
+    __shared__ uint32_t first_nan[D];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t lane = threadIdx.x & 63u, n = lane & 31u, half = lane >> 5;
 
@@ -244,8 +249,8 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
         limit = x < 0 ? 0 : (int32_t)x;
     }
     h8_t q[KK];
-    float qf, l = 0.0f, gap = 0.0f;
-    References ref = References::none();
+    float qf, l;
+    References ref;
     f16_t o[CB];
     {
         uint32_t row = seq.row0 + fr / p.G;
@@ -272,10 +277,6 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
             const uint32_t w = raw[i / 8][(i / 2) & 3];
             q[i / 8][i % 8] = (_Float16)(widen_el<BF16>((i & 1) ? w >> 16 : w & 0xffffu) * turned);
         }
-#pragma unroll
-        for (int c = 0; c < CB; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
     }
 
     // tokens that every row of the wave sees, and that some row does
@@ -293,127 +294,164 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
     if (part && first >= span.tiles) return;
     const uint32_t end = first + span.each < span.tiles ? first + span.each : span.tiles;
 
-    Stage<D, INT8, W> stage;
-    if (first < end) {
-        stage.entries(p, table, per_page, first * kTile);
-        stage.fetch(p, per_page, h, seq.tokens, first * kTile);
-        stage.store(lds + (first & 1) * Tile<D>::kBytes, info[first & 1]);
-    }
-    if (first + 1 < end) {
-        stage.entries(p, table, per_page, (first + 1) * kTile);
-        stage.fetch(p, per_page, h, seq.tokens, (first + 1) * kTile);
-        stage.entries(p, table, per_page, (first + 2) * kTile);
-    }
-    for (uint32_t j = first; j < end; ++j) {
-        __syncthreads();  // tile j is in LDS, the other buffer has been read
-        char* tile = lds + (j & 1) * Tile<D>::kBytes;
-        const StripInfo* at = info[j & 1];
-        const int32_t t0 = (int32_t)(j * kTile);
-        if (j + 1 < end) {
-            stage.store(lds + ((j + 1) & 1) * Tile<D>::kBytes, info[(j + 1) & 1]);
-            if (j + 2 < end) {
-                // (the entries of tile j + 2 came a tile ago)
-                stage.fetch(p, per_page, h, seq.tokens, t0 + 2 * kTile);
-                stage.entries(p, table, per_page, t0 + 3 * kTile);
-            }
+    // The walk. A causal one that ends with a NaN among its sums is made `again`, without
+    // the NaN among the values' codes (take_nan); a test for them at the causal edge, in
+    // one walk for all calls, costs up to 5% by the registers that it holds.
+    auto walk = [&](auto again) __attribute__((always_inline)) {
+        constexpr int AGAIN = decltype(again)::value;
+        float gap = 0.0f;
+        l = 0.0f;
+        ref = References::none();
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
+        Stage<D, INT8, W> stage;
+        if (first < end) {
+            stage.entries(p, table, per_page, first * kTile);
+            stage.fetch(p, per_page, h, seq.tokens, first * kTile);
+            stage.template store<AGAIN>(lds + (first & 1) * Tile<D>::kBytes, info[first & 1],
+                                        first_nan, first * kTile);
         }
-        if (t0 >= some) continue;
-
-        // The tile's operand blocks in the order of their MFMA: the keys of both
-        // blocks of tokens, then the values strip by strip. A ring of registers
-        // holds the next kRing of them, or each MFMA would wait for its LDS read (8192
-        // rows of 32 heads of 128: 616 us without, 597 with four, 594 with eight; 256
-        // channels leave registers for two: 865 us, 930 with four).
-        constexpr int kRing = D == 256 ? 2 : 4, kScores = 2 * KK;
-        h8_t ring[kRing];
-        auto operand = [&](int i) {
-            const int to = i < kScores ? i * Tile<D>::kKeyBlock
-                                       : Tile<D>::kKeys + (i - kScores) * 1024;
-            return *(const h8_t*)(tile + to + lane * 16);
-        };
-        f16_t s[2];
-#pragma unroll
-        for (int i = 0; i < kRing; ++i) ring[i] = operand(i);
-        __builtin_amdgcn_sched_group_barrier(0x100, kRing, 0);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[0][i] = s[1][i] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kScores; ++i) {
-            s[i / KK] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % kRing], q[i % KK], s[i / KK],
-                                                               0, 0, 0);
-            ring[i % kRing] = operand(i + kRing);
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if (first + 1 < end) {
+            stage.entries(p, table, per_page, (first + 1) * kTile);
+            stage.fetch(p, per_page, h, seq.tokens, (first + 1) * kTile);
+            stage.entries(p, table, per_page, (first + 2) * kTile);
         }
-        StripInfo st[kStrips];
-        int least = 16;
-#pragma unroll
-        for (int x = 0; x < kStrips; ++x) {
-            st[x] = at[x];
-            least = st[x].live < least ? st[x].live : least;
-        }
-        if (least < 16 || t0 + kTile > whole) {
-            // token 8 half + i of strip x
-#pragma unroll
-            for (int x = 0; x < kStrips; ++x) {
-                const int ahead = limit - t0 - 16 * x;
-                const int sees = (ahead < st[x].live ? ahead : st[x].live) - (int)(8 * half);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float y = s[x / 2][8 * (x & 1) + i];
-                    s[x / 2][8 * (x & 1) + i] = i < sees ? y : -__builtin_inff();
+        for (uint32_t j = first; j < end; ++j) {
+            __syncthreads();  // tile j is in LDS, the other buffer has been read
+            char* tile = lds + (j & 1) * Tile<D>::kBytes;
+            const StripInfo* at = info[j & 1];
+            const int32_t t0 = (int32_t)(j * kTile);
+            if (j + 1 < end) {
+                stage.template store<AGAIN>(lds + ((j + 1) & 1) * Tile<D>::kBytes,
+                                            info[(j + 1) & 1], first_nan, t0 + kTile);
+                if (j + 2 < end) {
+                    // (the entries of tile j + 2 came a tile ago)
+                    stage.fetch(p, per_page, h, seq.tokens, t0 + 2 * kTile);
+                    stage.entries(p, table, per_page, t0 + 3 * kTile);
                 }
             }
-        }
-        float fac[kStrips], product = -__builtin_inff(), lv = st[0].lv;
-        auto largest = [&](int x) {
-            float y = s[x / 2][8 * (x & 1)];
+            if (t0 >= some) continue;
+
+            // The tile's operand blocks in the order of their MFMA: the keys of both
+            // blocks of tokens, then the values strip by strip. A ring of registers
+            // holds the next kRing of them, or each MFMA would wait for its LDS read (8192
+            // rows of 32 heads of 128: 616 us without, 597 with four, 594 with eight; 256
+            // channels leave registers for two: 865 us, 930 with four).
+            constexpr int kRing = D == 256 ? 2 : 4, kScores = 2 * KK;
+            h8_t ring[kRing];
+            auto operand = [&](int i) {
+                const int to = i < kScores ? i * Tile<D>::kKeyBlock
+                                           : Tile<D>::kKeys + (i - kScores) * 1024;
+                return *(const h8_t*)(tile + to + lane * 16);
+            };
+            f16_t s[2];
 #pragma unroll
-            for (int i = 1; i < 8; ++i) y = fmaxf(y, s[x / 2][8 * (x & 1) + i]);
-            return y;
-        };
+            for (int i = 0; i < kRing; ++i) ring[i] = operand(i);
+            __builtin_amdgcn_sched_group_barrier(0x100, kRing, 0);
 #pragma unroll
-        for (int x = 0; x < kStrips; ++x) {
-            // (not 0: a masked score is -inf)
-            fac[x] = fmaxf(st[x].ks * qf, 1e-37f);
-            product = fmaxf(product, __builtin_fmaf(largest(x), fac[x], st[x].lv));
-            lv = fminf(lv, st[x].lv);
-        }
-        if (__any(ref.passes_or_holds(product, lv))) {
-            float weight = largest(0) * fac[0];
+            for (int i = 0; i < 16; ++i) s[0][i] = s[1][i] = 0.0f;
 #pragma unroll
-            for (int x = 1; x < kStrips; ++x) weight = fmaxf(weight, largest(x) * fac[x]);
-            product = fmaxf(product, xor_lanes(product, 32));
-            weight = fmaxf(weight, xor_lanes(weight, 32));
-            const References r = ref.moved_to(product, weight);
-            l *= r.s;
-#pragma unroll
-            for (int c = 0; c < CB; ++c) o[c] *= r.m;
-            gap = ref.gap();
-#pragma unroll
-            for (int x = 0; x < kStrips; ++x) ref.hold(st[x].lv, st[x].rvs);
-        }
-        h8_t pr[kStrips];
-        float weights = 0.0f;
-#pragma unroll
-        for (int x = 0; x < kStrips; ++x) {
-            const float off = st[x].lv - ref.m;
-            float sum;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float e = __builtin_amdgcn_exp2f(
-                    __builtin_fmaf(s[x / 2][8 * (x & 1) + i], fac[x], off));
-                sum = i ? sum + e : e;
-                pr[x][i] = (_Float16)e;
+            for (int i = 0; i < kScores; ++i) {
+                s[i / KK] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % kRing], q[i % KK], s[i / KK],
+                                                                   0, 0, 0);
+                ring[i % kRing] = operand(i + kRing);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
-            weights += sum * st[x].rvs;
-        }
-        l += weights * gap;
+            StripInfo st[kStrips];
+            int least = 16;
 #pragma unroll
-        for (int i = 0; i < kScores; ++i) {
-            const int c = i % CB;
-            o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % kRing], pr[i / CB], o[c], 0, 0, 0);
-            if (i + kRing < kScores) ring[i % kRing] = operand(kScores + i + kRing);
+            for (int x = 0; x < kStrips; ++x) {
+                st[x] = at[x];
+                least = st[x].live < least ? st[x].live : least;
+            }
+            if (least < 16 || t0 + kTile > whole) {
+                // token 8 half + i of strip x
+#pragma unroll
+                for (int x = 0; x < kStrips; ++x) {
+                    const int ahead = limit - t0 - 16 * x;
+                    const int sees = (ahead < st[x].live ? ahead : st[x].live) - (int)(8 * half);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float y = s[x / 2][8 * (x & 1) + i];
+                        s[x / 2][8 * (x & 1) + i] = i < sees ? y : -__builtin_inff();
+                    }
+                }
+            }
+            float fac[kStrips], product = -__builtin_inff(), lv = st[0].lv;
+            auto largest = [&](int x) {
+                float y = s[x / 2][8 * (x & 1)];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) y = fmaxf(y, s[x / 2][8 * (x & 1) + i]);
+                return y;
+            };
+#pragma unroll
+            for (int x = 0; x < kStrips; ++x) {
+                // (not 0: a masked score is -inf)
+                fac[x] = fmaxf(st[x].ks * qf, 1e-37f);
+                product = fmaxf(product, __builtin_fmaf(largest(x), fac[x], st[x].lv));
+                lv = fminf(lv, st[x].lv);
+            }
+            if (__any(ref.passes_or_holds(product, lv))) {
+                float weight = largest(0) * fac[0];
+#pragma unroll
+                for (int x = 1; x < kStrips; ++x) weight = fmaxf(weight, largest(x) * fac[x]);
+                product = fmaxf(product, xor_lanes(product, 32));
+                weight = fmaxf(weight, xor_lanes(weight, 32));
+                const References r = ref.moved_to(product, weight);
+                l *= r.s;
+#pragma unroll
+                for (int c = 0; c < CB; ++c) o[c] *= r.m;
+                gap = ref.gap();
+#pragma unroll
+                for (int x = 0; x < kStrips; ++x) ref.hold(st[x].lv, st[x].rvs);
+            }
+            h8_t pr[kStrips];
+            float weights = 0.0f;
+#pragma unroll
+            for (int x = 0; x < kStrips; ++x) {
+                const float off = st[x].lv - ref.m;
+                float sum;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(
+                        __builtin_fmaf(s[x / 2][8 * (x & 1) + i], fac[x], off));
+                    sum = i ? sum + e : e;
+                    pr[x][i] = (_Float16)e;
+                }
+                weights += sum * st[x].rvs;
+            }
+            l += weights * gap;
+#pragma unroll
+            for (int i = 0; i < kScores; ++i) {
+                const int c = i % CB;
+                o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % kRing], pr[i / CB], o[c], 0, 0, 0);
+                if (i + kRing < kScores) ring[i % kRing] = operand(kScores + i + kRing);
+            }
+        }
+    };
+    walk(Const<0>());
+    const bool nan_matters = !INT8 && p.causal;
+    if (nan_matters) {
+        bool some = false;
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) some |= o[c][i] != o[c][i];
+        for (uint32_t i = threadIdx.x; i < D; i += 64 * W) first_nan[i] = kNoToken;
+        if (__syncthreads_or(some)) {
+            walk(Const<1>());
+#pragma unroll
+            for (int c = 0; c < CB; ++c)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const u4_t t = *(const u4_t*)&first_nan[32 * c + 8 * x + 4 * half];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (t[i] < (uint32_t)limit) o[c][4 * x + i] = __builtin_nanf("");
+                }
         }
     }
 

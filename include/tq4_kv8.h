@@ -113,8 +113,9 @@ int tq4_kv8_reshape_and_cache(void* stream, int element_type, int code_type, con
  * same shape, contiguous; q head j reads kv head j / (num_heads /
  * num_kv_heads). block_tables [num_seqs][max_blocks_per_seq]; context_lens
  * [num_seqs] (held in [0, max_blocks_per_seq * S]). A token whose table entry
- * names no page, or past its context, contributes nothing, whatever its bytes
- * are; a row that sees no token is 0.
+ * names no page, past its context, or behind what a causal row sees contributes
+ * nothing, whatever its bytes are (a NaN code of another writer's among them); a
+ * row that sees no token is 0.
  *
  * The decode: one row a sequence (row b = sequence b).
  * num_splits, at most TQ4_KV8_MAX_SPLITS: the parts that each sequence's tokens
