@@ -143,7 +143,8 @@ def paged_plan(context_lens, query_lens, block_tables, free_pages, free_state, s
     granted and release [B], block_tables [B][max_blocks], free_pages [P] (the
     ring of free pages), free_state {head, count}, slot_mapping and positions
     [rows], cu_seqlens [B + 1]. new_context_lens and new_free_state None: in
-    place."""
+    place. The table entries of a released context and the ring's free entries
+    all have to name pages: one that names none is handed on like a page."""
     what = "paged_plan"
     f = _fast()
     if f is not None and _done(f.paged_plan(

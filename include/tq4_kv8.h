@@ -51,7 +51,11 @@ extern "C" {
  *      ceil(c/S) pages back, in request order, to the ring's end, and its
  *      context becomes empty. Pages given back serve the next call on; a page
  *      that would not fit into the ring (more pages than the pool has) is
- *      dropped.
+ *      dropped. All ceil(c/S) entries have to name pages, as the ring's free
+ *      entries have to: one that names none is counted and handed on like a
+ *      page, and the rows that a later request is granted in it have slot -1. A
+ *      caller that takes pages out of a request's table gives the others back
+ *      itself, or shortens the context to those in front, before it releases it.
  *   2. In request order, b needs w = ceil((c + n)/S) - ceil(c/S) pages. It is
  *      granted when its context fits the table and its rows fit max_tokens,
  *      and w is 0 or the pages needed up to and with it, by requests that fit,
