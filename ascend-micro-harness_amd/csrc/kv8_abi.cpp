@@ -43,7 +43,7 @@ int cache_checks(int element_type, int code_type, uint32_t num_kv_heads, uint32_
 // How a call's work is cut (kv8_decode.hip): K parts a sequence, or 0: streamed
 // over `groups` workgroups.
 struct Cut {
-    uint32_t K, groups, least;
+    uint32_t K, groups;
 };
 
 uint64_t tiles_of(uint64_t max_q, uint64_t group)
@@ -54,22 +54,24 @@ uint64_t tiles_of(uint64_t max_q, uint64_t group)
 // The choice between one workgroup an item (no second kernel), even parts, and
 // streaming, which keeps all CUs busy whatever the lengths are. A workgroup walks cap
 // tokens in cap * d * 0.0375 ns, all items together cost their bytes at 4.9 TB/s
-// (3.9 with half the CUs) and a second kernel 4 us. Heads of 128, 8 KV heads, us for
-// one workgroup / parts / streamed:
-//   4 sequences of 300..1500 tokens   10.8 /  8.5 / 11.0
-//   16 of 300..1500                   10.8 / 12.6 / 17.7
-//   16 of 300..4099                   22.5 / 19.2 / 25.7
-//   16 of 500..20000                  128  / 84   / 72     parts of 10000: uneven
-//   32 of 500..4096                   35.8 / 41.5 / 38.6
-//   128 of 500..4096                  127  / 125  / 116    (even ones 190 / 211 / 212)
-// Parts: one workgroup a CU (one sequence of 4096: 16 / 32 / 64 parts 8.5 / 7.8 / 8.7
-// us; of 65536 32 / 64 29.4 / 30.5), of 128 tokens at least, and no more than 64, or
-// 128, where the join's share grows (2 heads of 65536: 64 / 128 parts 12.8 / 13.3; of
-// 256 channels 20.8 / 19.1). A streamed workgroup has four units at least.
+// (3.9 with half the CUs) and a second kernel 4 us. Heads of 128, 8 KV heads, 4 rows
+// each, tables as wide as the longest context, us for one workgroup / parts / streamed:
+//   4 sequences of 300..1500 tokens   11.8 /  8.9 / 12.4
+//   16 of 300..1500                   12.2 / 13.2 / 18.5
+//   16 of 300..4099                   24.0 / 21.9 / 24.7
+//   16 of 500..20000                  132  / 85   / 79     parts of 10000: uneven
+//   32 of 500..4096                   35.4 / 40.8 / 36.9
+//   128 of 500..4096                  131  / 133  / 121    (3000..4096: 172 / 182 / 176)
+// cap is the table's tokens, so in a table far wider than its contexts the choice is
+// that of longer ones (in one of 8192 tokens and more, 16 of 600..2048: 14.5 -> 19.7).
+// Parts: one workgroup a CU (one sequence of 4096: 16 / 32 / 64 parts 9.4 / 9.0 / 9.9
+// us; of 65536 32 / 64 31.5 / 32.4), of 128 of the table's tokens at least, and no more
+// than 64, or 128, where the join's share grows (2 heads of 65536: 64 / 128 parts 15.2 /
+// 15.5; of 256 channels 23.1 / 21.8).
 Cut cut_rule(uint32_t d, uint64_t seqs, uint64_t heads, uint64_t tiles, uint64_t cap,
              uint32_t num_splits)
 {
-    Cut c{num_splits, 0, 4};
+    Cut c{num_splits, 0};
     if (num_splits) return c;
     c.groups = 256u * (uint32_t)tq4::kKv8GroupsPerCu((int)d);
     uint64_t items = mul(seqs, heads, tiles);
@@ -110,11 +112,16 @@ size_t record_bytes(const Cut& c, uint64_t items, uint32_t rec_rows, uint32_t d)
 // and more in LDS. Up to 32 rows it is the better; behind, while its tiles are at
 // most three times those that the GPU holds at once, and its tiles times a table's
 // tokens are few. Measured with 4 rows of 8 KV heads of 128 a token (us, decode
-// kernel against the other):
-//   32 rows   16 sequences of 500..4000 tokens  32, 42;  of 500..1000   10, 24
-//   64 rows   the same                          43, 48;  256 rows of 500..4000  105, 107
-//   512 rows  4 sequences of 1000 tokens        28, 42;  1024 rows      48, 45
-//   256 rows  1 sequence of 4096                22, 36;  512 rows of 32768     156, 97
+// kernel against the other; rows of a sequence and KV head):
+//   32 rows   16 sequences of 500..4000 tokens  26, 40;   of 500..1000   11, 23
+//   64 rows   the same                          44, 50;   17, 28
+//   256 rows  the same                         156, 92;   47, 34
+//   512 rows  4 sequences of 1000 tokens        27, 32;   1024 rows      45, 33
+//   256 rows  1 sequence of 4096                19, 34;   of 32768       82, 63
+// The product is no sharp line: at 2.0 million 1536 rows of one sequence of 2600 take
+// 41, 46, but 192 rows of 4 of 5200 take 84, 41. Heads of 256: 256 rows of one of 4096
+// (0.5 million) 33, 51; 64 rows of 16 of 500..1000 35, 57; 192 rows of one of 16384 (1.6
+// million) 85, 76; 384 rows of 4 of 2600 (2.0 million) 154, 87.
 bool few_rows(uint32_t d, uint64_t num_rows, uint64_t seqs, uint64_t heads, uint64_t group,
               uint64_t max_q, uint64_t cap)
 {
@@ -124,14 +131,17 @@ bool few_rows(uint32_t d, uint64_t num_rows, uint64_t seqs, uint64_t heads, uint
     if (all > num_rows * group / tq4::kKv8Rows + seqs) all = num_rows * group / tq4::kKv8Rows + seqs;
     all = mul(all, heads);
     return mul(heads, tiles) <= 65535u && all <= 768ull * tq4::kKv8GroupsPerCu((int)d) &&
-           mul(all, cap) <= (d == 256 && seqs > 1 ? 1310720u : 2250000u);
+           mul(all, cap) <= (d == 256 ? 1310720u : 2250000u);
 }
 
 // The parts that a prefill's row tiles cut their tokens into: with fewer row tiles
-// than the CUs hold at once, as many as fill them, of 256 tokens at least and while
-// a part's records (written and read: 8 bytes an element at 2.4 TB/s) cost less than
-// it saves (a tile of 64 tokens takes 2.2 us with eight waves, 1.3 with four): 512
-// rows of 8 KV heads of 128 over 4096 tokens 36 us in 11 parts, 30 in 8.
+// than the CUs hold at once, as many as fill them, of 256 of the table's tokens at
+// least and while a part's records (written and read: 8 bytes an element at 2.4 TB/s)
+// cost less than it saves (a tile of 64 tokens is taken for 2.2 us with eight waves, 1.3
+// with four). 1024 rows of 8 KV heads of 128 over 4096 tokens: 121 us in one part, 45 in
+// 6, 43 in 8 (taken), 56 in 11; 512 over 16384: 450, 64 in 11 (taken), 58 in 16. Shorter
+// contexts in a wide table have shorter parts (512 rows over 512 tokens: 8 us by the
+// decode kernel in a table of 8192, 27 in one of 32768).
 uint32_t prefill_parts(uint32_t d, uint64_t num_rows, uint64_t seqs, uint64_t heads,
                        uint64_t group, uint64_t max_q, uint64_t cap)
 {
@@ -211,7 +221,6 @@ tq4::Kv8AttnParams make(const void* q, const void* kc, const void* vc, const flo
     p.M = max_blocks;
     p.K = cut.K;
     p.groups = cut.groups;
-    p.least = cut.least;
     p.max_q = max_q;
     p.causal = causal;
     p.scale = scale;
@@ -361,7 +370,7 @@ size_t tq4_kv8_prefill_workspace_bytes(uint32_t num_rows, uint32_t num_seqs, uin
     if (!few_rows(head_size, num_rows, num_seqs, num_kv_heads, group, max_query_len, cap)) {
         const uint32_t k = prefill_parts(head_size, num_rows, num_seqs, num_kv_heads, group,
                                          max_query_len, cap);
-        return k == 1 ? 0 : record_bytes(Cut{k, 0, 0}, mul(num_rows, num_heads), 1, head_size);
+        return k == 1 ? 0 : record_bytes(Cut{k, 0}, mul(num_rows, num_heads), 1, head_size);
     }
     const Cut c =
         cut_rule(head_size, num_seqs, num_kv_heads, tiles_of(max_query_len, group), cap, 0);
@@ -407,7 +416,7 @@ int tq4_kv8_paged_prefill(void* stream, int element_type, int code_type, const v
             mul(num_rows, num_heads) > kMaxGroups)
             return TQ4_ERR_RANGE;
         if (!room) return TQ4_ERR_WORKSPACE;
-        tq4::Kv8AttnParams p = args(Cut{k, 0, 0});
+        tq4::Kv8AttnParams p = args(Cut{k, 0});
         p.stats = p.acc + (uint64_t)num_rows * num_heads * k * head_size;
         return launched(tq4::launch_kv8_prefill((hipStream_t)stream, element_type,
                                                 code_type == TQ4_KV8_INT8, p));

@@ -158,7 +158,7 @@ struct Sequence : SequenceBase {
 __device__ __forceinline__ uint32_t quota_of(const Kv8AttnParams& p, uint32_t total)
 {
     const uint32_t q = ((total + p.groups - 1) / p.groups + kWaves - 1) / kWaves * kWaves;
-    return q > p.least ? q : p.least;
+    return q ? q : kWaves;  // a unit a wave at least
 }
 __device__ __forceinline__ uint32_t part_units(const Kv8AttnParams& p, uint32_t units)
 {

@@ -46,8 +46,8 @@ struct Kv8AttnParams {
     void* out;
     uint64_t q_stride;
     uint32_t rows, B, Hq, Hkv, G, D, S, P, M;
-    uint32_t K;              // parts of a sequence; 0: streamed over `groups`
-    uint32_t groups, least;  // workgroups, and units that one takes at least
+    uint32_t K;       // parts of a sequence; 0: streamed over `groups`
+    uint32_t groups;  // workgroups
     uint32_t rec_rows;
     uint32_t max_q;
     int causal;
@@ -56,10 +56,10 @@ struct Kv8AttnParams {
 // Waves of a prefill workgroup, 32 rows each (kv8_prefill.hip), for so many rows of a
 // (sequence, kv head) over tables of `cap` tokens, and the workgroups that the CUs
 // hold at once. Eight waves widen a tile for twice the rows (8192 rows x 32 heads of
-// 128: 619 us against 651), four are the more balanced where there are few tiles (2048
-// rows: 72 us against 81; 1000: 37, 42); heads of 64 run better as three workgroups of
-// four a CU (376 us against 418 with eight waves), and 256 channels fill a wave's
-// registers and a CU's LDS with four.
+// 128: 568 us, 605 with four; 4000 rows 151, 175), four are the more balanced where there
+// are few tiles (3000 rows: 99 us, 101 with eight; 2048: 62, 68; 1000: 33, 37); a tile of
+// 64 channels has pieces for four, and 256 channels fill a wave's registers and a CU's
+// LDS with four.
 inline uint32_t kv8_prefill_waves(uint32_t d, uint64_t rows, uint64_t cap)
 {
     return d == 128 && rows > 128 && cap > 2048 ? 8 : 4;

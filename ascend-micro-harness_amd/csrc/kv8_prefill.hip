@@ -67,7 +67,8 @@ struct StripInfo {
 template <int D, int INT8, int W>
 struct Stage {
     static constexpr int kThreads = 64 * W, kPieces = 4 * D;
-    static constexpr int N = (kPieces + kThreads - 1) / kThreads;
+    static constexpr int N = kPieces / kThreads;
+    static_assert(kPieces % kThreads == 0, "every thread brings N pieces");
     u4_t k[N], v[N];
     int live[N];   // live tokens of the pieces' strips
     int32_t e[N];  // the next fetch's block-table entries, as they come from memory
@@ -78,11 +79,7 @@ struct Stage {
 
     __device__ __forceinline__ Stage() { asm("v_mov_b32 %0, 0" : "=v"(zero)); }
 
-    // (a wave too many brings another's pieces, and does not store them)
-    static __device__ __forceinline__ uint32_t piece(int r)
-    {
-        return (r * kThreads + threadIdx.x) % kPieces;
-    }
+    static __device__ __forceinline__ uint32_t piece(int r) { return r * kThreads + threadIdx.x; }
     static __device__ __forceinline__ uint32_t strip_of(int r)
     {
         return __builtin_amdgcn_readfirstlane(piece(r) / D);
@@ -148,7 +145,6 @@ struct Stage {
     {
 #pragma unroll
         for (int r = 0; r < N; ++r) {
-            if (N * kThreads > kPieces && r * kThreads + threadIdx.x >= kPieces) break;
             const uint32_t u = piece(r);
             {
                 const uint32_t token = u / (D / 16), block = token / 32, x = token % 32;
