@@ -22,9 +22,9 @@
 // (2^-11 relative) and v's codes are exact in it; out is rounded once.
 //
 // The cache's bytes bound it, then the second kernel: 64 sequences of 512..8192
-// tokens (552 MB) 107 us, 5.2 TB/s of 5.6 that reading the strips alone reaches; one
-// of 65536 tokens of 2 heads of 256 (67 MB) 17 us and 5 to join 128 parts; one of
-// 4096 5 and 3. A unit of 64 tokens keeps a lane's loads 16 bytes wide and a
+// tokens (552 MB) 109 us, 5.05 TB/s of 5.6 that reading the strips alone reaches; one
+// of 65536 tokens of 2 heads of 256 (67 MB) 18 us and 6 to join 128 parts; one of
+// 4096 6 and 4. A unit of 64 tokens keeps a lane's loads 16 bytes wide and a
 // strip's scale one a lane; the loads run a unit ahead in the registers that the
 // products just freed (a second set of registers spills at 256 channels).
 #include <hip/hip_runtime.h>

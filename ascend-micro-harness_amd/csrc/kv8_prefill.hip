@@ -16,12 +16,13 @@
 // Two LDS buffers: tile j is computed while tile j + 1 is widened into the other
 // and tile j + 2 comes from memory.
 //
-// Arithmetic bounds it: 8192 causal rows of 32 heads of 128 (8 KV heads) 557 us, 987
-// TFLOP/s where a library product of f16 matrices reaches 1336; 64 channels 355 us,
-// 775; 256 800 us, 690 (its 32 rows fill a wave's registers: one wave a SIMD). (Cards
-// and their clocks differ by 6%.) An earlier form, of 616 us, took 426 without the
-// softmax and the widening, which added about 100 each; a ring of operand blocks and
-// table entries that nothing waits for made up the difference. Issue order otherwise
+// Arithmetic bounds it: 8192 causal rows of 32 heads of 128 (8 KV heads) 556 us, 988
+// TFLOP/s where a library product of f16 matrices reaches 1284 to 1336; of 32 heads of
+// 64 355 us, 775; of 16 heads of 256 808 us, 681 (its 32 rows fill a wave's registers:
+// one wave a SIMD). (Cards and their clocks differ by up to 12%.) An earlier form, of
+// 616 us, took 426 without the softmax and the widening, which added about 100 each; a
+// ring of operand blocks and table entries that nothing waits for made up the
+// difference. Issue order otherwise
 // is not what holds it: priorities for one of a SIMD's two waves, a wave half a tile
 // behind the other, and a tile's softmax beside the next one's scores in one wave all
 // took as long or longer. 64 rows a wave halve the LDS reads, but their sums move
@@ -332,9 +333,10 @@ __global__ __launch_bounds__(64 * W, D < 256 ? 2 : 1) void kv8_prefill(Kv8AttnPa
 
             // The tile's operand blocks in the order of their MFMA: the keys of both
             // blocks of tokens, then the values strip by strip. A ring of registers
-            // holds the next kRing of them, or each MFMA would wait for its LDS read (8192
-            // rows of 32 heads of 128: 616 us without, 597 with four, 594 with eight; 256
-            // channels leave registers for two: 865 us, 930 with four).
+            // holds the next kRing of them, or each MFMA would wait for its LDS read
+            // (8192 rows of 32 heads of 128, when it was added: 616 us without, 597 with
+            // four, 594 with eight; 256 channels leave registers for two: 865 us, 930
+            // with four).
             constexpr int kRing = D == 256 ? 2 : 4, kScores = 2 * KK;
             h8_t ring[kRing];
             auto operand = [&](int i) {
