@@ -356,7 +356,7 @@ int tq4_kv8_paged_decode(void* stream, int element_type, int code_type, const vo
         (hipStream_t)stream, element_type, code_type == TQ4_KV8_INT8,
         make(q, key_cache, value_cache, scale_cache, block_tables, context_lens, nullptr, out,
              q_stride, num_seqs, num_seqs, num_heads, num_kv_heads, head_size, block_size,
-             num_blocks, max_blocks_per_seq, 1, 1, scale, s, workspace)));
+             num_blocks, max_blocks_per_seq, 1, 0, scale, s, workspace)));
 }
 
 size_t tq4_kv8_prefill_workspace_bytes(uint32_t num_rows, uint32_t num_seqs, uint32_t num_heads,

@@ -10,8 +10,8 @@
 // Latency bounds it: a round trip for the lengths, the scans, one for the table
 // or ring entries, the stores. So one launch where it can be: each workgroup
 // makes the scans for itself (a thread a request, the records in LDS) and fills
-// its share of rows and tables. 64 requests 4.6 us, 1000 with 16000 rows 8.0 (three
-// launches: 12); 0.55 MB, so a launch is the floor of both.
+// its share of rows and tables. 64 requests 4.5 us, 1000 with 61000 rows 8.0 (three
+// launches: 12; in place, in two: 15); 0.55 MB, so a launch is the floor of both.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

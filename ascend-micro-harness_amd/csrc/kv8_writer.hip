@@ -17,7 +17,9 @@
 //
 // Memory bounds the prompts: 16384 rows of 8 heads of 128 24.3 us, 4.1 TB/s of the
 // 4.9 that a copy reaches (a wave a whole page: 34 us, its strips one after the
-// other). 64 single rows 3.7 us, a launch; a wave a row instead of 16 lanes 6.0.
+// other). 64 single rows 3.8 us, a launch; a wave a row instead of 16 lanes 6.0. Pages
+// whose scale grows are moved one after the other by the wave that wrote their row: where
+// all 512 (page, head) pairs of 64 rows grow, 5 / 22 / 45 us more in pages of 16 / 64 / 128.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
